@@ -17,7 +17,7 @@ import torch
 own = False
 
 GROUP = 32  # values of one head that share a scale and a zero point
-FP16_MAX = 65504.0
+HELD_MAX = 57344.0  # larger magnitudes are held as this
 DTYPES = {
     "bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32,
 }
@@ -384,7 +384,7 @@ def _quantize(x):
     range, both held in 16 bits; a code is the nearest whole number of scales
     above the zero point, a tie going to the even one. In 64 bits, since the
     codes are decided at borders."""
-    x = x.double().clamp(-FP16_MAX, FP16_MAX)
+    x = x.double().clamp(-HELD_MAX, HELD_MAX)
     x = x.unflatten(-1, (-1, GROUP))
     zero = x.amin(-1).half()
     scale = ((x.amax(-1) - zero.double()) / 15.0).half()
@@ -585,7 +585,7 @@ def _exact_held(x):
     out = torch.empty(x.shape, dtype=torch.float64, device=x.device)
     for low in range(0, x.shape[-1], GROUP):
         part = x[..., low:low + GROUP].double()
-        part = part.clamp(min=-FP16_MAX, max=FP16_MAX)
+        part = part.clamp(min=-HELD_MAX, max=HELD_MAX)
         zero = part.min(-1, keepdim=True)[0].half().double()
         scale = ((part.max(-1, keepdim=True)[0] - zero) / 15).half().double()
         code = torch.round((part - zero) / scale.clamp(min=1e-300))
