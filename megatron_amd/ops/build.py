@@ -37,13 +37,17 @@ def build(verbose: bool = True, force: bool = False) -> str:
         for f in os.listdir(CSRC)
         if f.endswith(".hip") or f.endswith(".cpp")
     )
-    common_h = os.path.join(CSRC, "common.h")
+    # what every object hangs on: the flags in this file, and common.h
+    shared = max(os.path.getmtime(os.path.join(CSRC, "common.h")),
+                 os.path.getmtime(os.path.abspath(__file__)))
 
     cflags = [
         f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC",
         "-DTORCH_EXTENSION_NAME=_C", "-D__HIP_PLATFORM_AMD__=1",
         "-DUSE_ROCM=1", "-D_GLIBCXX_USE_CXX11_ABI=1",
         "-Wno-unused-result",
+        # scalar fp32 only: some packed fp32 forms have returned wrong results
+        "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     ]
     for p in inc_paths:
         cflags.append(f"-I{p}")
@@ -58,7 +62,7 @@ def build(verbose: bool = True, force: bool = False) -> str:
         objs.append(obj)
         need = force or not os.path.exists(obj) or (
             os.path.getmtime(obj) < os.path.getmtime(src)
-            or os.path.getmtime(obj) < os.path.getmtime(common_h)
+            or os.path.getmtime(obj) < shared
         )
         if need:
             cmd = ["hipcc", "-c", "-x", "hip", src, "-o", obj] + cflags

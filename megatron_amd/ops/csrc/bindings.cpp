@@ -100,6 +100,37 @@ std::vector<torch::Tensor> flash_attn_bwd(torch::Tensor dout, torch::Tensor q,
                                           double dropout_p, int64_t drop_seed,
                                           int64_t drop_offset);
 
+// rotary.hip
+std::vector<torch::Tensor> rotary_apply(
+    torch::Tensor q, c10::optional<torch::Tensor> k, torch::Tensor cos,
+    torch::Tensor sin, c10::optional<torch::Tensor> positions,
+    bool interleaved, bool inverse);
+
+// quant_kv.hip
+c10::optional<torch::Tensor> quant_kv_append(
+    std::vector<torch::Tensor> buffers, int64_t capacity, torch::Tensor key,
+    torch::Tensor value, c10::optional<torch::Tensor> start, int64_t start_s,
+    c10::optional<torch::Tensor> query, c10::optional<torch::Tensor> cos,
+    c10::optional<torch::Tensor> sin, bool interleaved);
+std::vector<torch::Tensor> quant_kv_dequantize(
+    std::vector<torch::Tensor> buffers, int64_t capacity,
+    c10::optional<torch::Tensor> start, int64_t start_s, int64_t length,
+    bool bf16);
+torch::Tensor quant_kv_attention(std::vector<torch::Tensor> buffers,
+                                 int64_t capacity, torch::Tensor query,
+                                 c10::optional<torch::Tensor> start,
+                                 int64_t start_s, double scale,
+                                 int64_t window, int64_t sinks);
+
+// sample.hip
+torch::Tensor sample_tokens(torch::Tensor logits, torch::Tensor uniform,
+                            c10::optional<torch::Tensor> temperature,
+                            c10::optional<torch::Tensor> top_k,
+                            c10::optional<torch::Tensor> top_p,
+                            c10::optional<torch::Tensor> min_p,
+                            double temperature_s, int64_t top_k_s,
+                            double top_p_s, double min_p_s);
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("rmsnorm_fwd", &rmsnorm_fwd);
   m.def("wgrad_gemm_hand", &wgrad_gemm_hand);
@@ -131,6 +162,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("build_sample_idx", &build_sample_idx);
   m.def("build_blending_indices", &build_blending_indices);
   m.def("fp8_quantize", &fp8_quantize);
+  m.def("rotary_apply", &rotary_apply);
+  m.def("quant_kv_append", &quant_kv_append);
+  m.def("quant_kv_dequantize", &quant_kv_dequantize);
+  m.def("quant_kv_attention", &quant_kv_attention);
+  m.def("sample_tokens", &sample_tokens);
   m.def("flash_attn_fwd", &flash_attn_fwd, py::arg("q"),
         py::arg("k"), py::arg("v"), py::arg("causal"),
         py::arg("softmax_scale"), py::arg("window_size"),

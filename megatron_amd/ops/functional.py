@@ -369,6 +369,109 @@ def apply_rope(x, cos, sin):
 
 
 # ---------------------------------------------------------------------------
+# Rotary embedding in any layout: interleaved or half pairs, part of the head,
+# a position per token, query and key in one launch (csrc/rotary.hip).
+
+def rotate_reference(x, cos, sin, interleaved):
+    """x [s, b, n, h] turned by cos, sin [s, b or 1, r] in their own type,
+    rounded once; values past 2r are left as they are."""
+    r = cos.shape[-1]
+    c, s = cos.unsqueeze(2), sin.unsqueeze(2)
+    t, rest = x[..., : 2 * r].to(cos.dtype), x[..., 2 * r:]
+    if interleaved:
+        x1, x2 = t[..., 0::2], t[..., 1::2]
+        y = torch.stack([x1 * c - x2 * s, x2 * c + x1 * s], dim=-1).flatten(-2)
+    else:
+        x1, x2 = t[..., :r], t[..., r:]
+        y = torch.cat([x1 * c - x2 * s, x2 * c + x1 * s], dim=-1)
+    return torch.cat([y.to(x.dtype), rest], dim=-1)
+
+
+class RotaryFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, query, key, cos, sin, positions, interleaved, inverse):
+        ctx.save_for_backward(cos, sin, positions)
+        ctx.mode = (interleaved, inverse)
+        ctx.set_materialize_grads(False)
+        ext = _C(query)
+        if ext is not None:
+            # the kernel reads strided views with a dense head_dim
+            q, k = (t if t is None or t.stride(-1) == 1 else t.contiguous()
+                    for t in (query, key))
+            out = ext.rotary_apply(q, k, cos, sin, positions, interleaved,
+                                   inverse)
+            return out[0], (out[1] if key is not None else None)
+        if positions is None:
+            c, s = (t[: query.shape[0]].unsqueeze(1) for t in (cos, sin))
+        else:
+            c, s = (t[positions.t()] for t in (cos, sin))
+        if inverse:
+            s = -s
+        return (rotate_reference(query, c, s, interleaved),
+                rotate_reference(key, c, s, interleaved)
+                if key is not None else None)
+
+    @staticmethod
+    def backward(ctx, dq, dk):
+        # the transpose of the rotation: the same with the angle negated
+        cos, sin, positions = ctx.saved_tensors
+        interleaved, inverse = ctx.mode
+        rest = (cos, sin, positions, interleaved, not inverse)
+        if dq is None and dk is not None:
+            dk, _ = RotaryFunction.apply(dk, None, *rest)
+        elif dq is not None:
+            dq, dk = RotaryFunction.apply(dq, dk, *rest)
+        return dq, dk, None, None, None, None, None
+
+
+def rotary_embedding(query, key, cos, sin, positions=None, interleaved=True):
+    """Rotate query [s, b, n, h] and key [s, b, nkv, h] (or None) by their
+    tokens' positions; returns both.
+
+    cos, sin: fp32 [S, r] with r <= h / 2, from precompute_rotary_tables
+    (models/rope.py): the first 2r values of a head are rotated, the others
+    pass through. positions: int64 [b, s], rows of the tables; None means
+    0..s-1 in every sequence. interleaved: pairs are (2j, 2j + 1), else
+    (j, j + r). Positions outside the tables are refused on the CPU and give
+    NaN on the GPU. Differentiable in query and key."""
+    if query.dim() != 4:
+        raise ValueError("query must be [s, b, heads, head_dim]")
+    s, b, _, h = query.shape
+    if query.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise ValueError(f"rotary_embedding takes fp32, bf16 or fp16, not "
+                         f"{query.dtype}")
+    if key is not None and (
+            key.dim() != 4 or key.shape[:2] != query.shape[:2]
+            or key.shape[3] != h or key.dtype != query.dtype
+            or key.device != query.device):
+        raise ValueError("key must match the query but for its heads")
+    for t in (cos, sin):
+        if (t.dim() != 2 or t.dtype != torch.float32 or t.shape != cos.shape
+                or t.device != query.device
+                or not 1 <= t.shape[1] <= h // 2):
+            raise ValueError("cos and sin must be float32 [positions, up to "
+                             f"{h // 2}] on {query.device}")
+        if t.requires_grad:
+            raise ValueError("cos and sin have no gradient")
+    if positions is None:
+        if cos.shape[0] < s:
+            raise ValueError(f"tables of {cos.shape[0]} positions for {s} "
+                             "tokens")
+    else:
+        if (positions.shape != (b, s) or positions.dtype != torch.int64
+                or positions.device != query.device):
+            raise ValueError(f"positions must be int64 [{b}, {s}] on "
+                             f"{query.device}")
+        if not positions.is_cuda and positions.numel() and (
+                int(positions.min()) < 0
+                or int(positions.max()) >= cos.shape[0]):
+            raise ValueError("a position lies outside the tables")
+    return RotaryFunction.apply(query, key, cos.contiguous(),
+                                sin.contiguous(), positions, interleaved,
+                                False)
+
+
+# ---------------------------------------------------------------------------
 # bias + dropout + residual add (reference transformer.py:596-609)
 
 class BiasDropoutAdd(torch.autograd.Function):
@@ -683,3 +786,106 @@ class FusedQKVSplitRope(torch.autograd.Function):
 
 def fused_qkv_split_rope(mixed, cos, sin, np_, nkv, hn):
     return FusedQKVSplitRope.apply(mixed, cos, sin, np_, nkv, hn)
+
+
+# ---------------------------------------------------------------------------
+# Next tokens from filtered logits and given uniform numbers
+# (csrc/sample.hip).
+
+def sample_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=0.0,
+                  min_p=0.0):
+    """Draw one token per row of logits [b, v]; int64 [b].
+
+    uniform: float32 [b] in [0, 1). The settings are numbers, or tensors [b]
+    for a setting per row (float32; top_k int64). Tokens are ordered by logit,
+    equal ones by index. Of the weights exp((x - max) / temperature), top_k
+    keeps the first k tokens (0: all), top_p of those each whose predecessors
+    weigh at most top_p of them all (0 or 1: all), min_p those that weigh at
+    least min_p times the largest. The token drawn is the first index whose
+    kept weights up to it exceed uniform times all kept weights. temperature 0
+    takes the largest logit, the lowest index of equal ones.
+
+    A row with a NaN, or without a logit above -inf, gives -1."""
+    if logits.dim() != 2 or logits.shape[1] < 1:
+        raise ValueError("logits must be [b, vocabulary]")
+    b, v = logits.shape
+    if v > 1 << 20:
+        raise ValueError("at most 2^20 tokens")
+    if logits.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise ValueError(f"sample_tokens takes fp32, bf16 or fp16, not "
+                         f"{logits.dtype}")
+    settings = dict(uniform=uniform, temperature=temperature, top_k=top_k,
+                    top_p=top_p, min_p=min_p)
+    rows, numbers = {}, {}
+    for name, x in settings.items():
+        want = torch.int64 if name == "top_k" else torch.float32
+        if isinstance(x, torch.Tensor):
+            if (x.shape != (b,) or x.dtype != want
+                    or x.device != logits.device):
+                raise ValueError(f"{name} must be a number or a {want} "
+                                 f"tensor [{b}] on {logits.device}")
+            rows[name], numbers[name] = x.contiguous(), 0
+        elif name == "uniform":
+            raise ValueError("uniform must be a tensor")
+        else:
+            rows[name] = None
+            numbers[name] = int(x) if name == "top_k" else float(x)
+    if not 0.0 <= numbers["temperature"] < math.inf:
+        raise ValueError("temperature must be finite and not negative")
+    if numbers["top_k"] < 0:
+        raise ValueError("top_k must not be negative")
+    for name in ("top_p", "min_p"):
+        if not 0.0 <= numbers[name] <= 1.0:
+            raise ValueError(f"{name} must be in 0..1")
+    if logits.requires_grad and torch.is_grad_enabled():
+        logits = logits.detach()  # a drawn token has no gradient
+    ext = _C(logits)
+    if ext is not None:
+        if logits.stride(1) != 1:
+            logits = logits.contiguous()
+        return ext.sample_tokens(
+            logits, rows["uniform"], rows["temperature"], rows["top_k"],
+            rows["top_p"], rows["min_p"], numbers["temperature"],
+            numbers["top_k"], numbers["top_p"], numbers["min_p"])
+
+    def setting(name):
+        if rows[name] is not None:
+            return rows[name].double()[:, None]
+        return torch.full((b, 1), numbers[name], dtype=torch.float64)
+
+    return _sample_reference(logits.double(), *(
+        setting(x) for x in ("temperature", "top_k", "top_p", "min_p")),
+        uniform.double()[:, None])
+
+
+def _sample_reference(x, temperature, top_k, top_p, min_p, uniform):
+    top = x.amax(-1, keepdim=True)
+    greedy = ~(temperature > 0)
+    top_k = torch.where(greedy, torch.ones_like(top_k), top_k)
+    temperature = torch.where(greedy, torch.ones_like(temperature),
+                              temperature).clamp(max=1e30)
+    weight = torch.where(x == top, torch.ones_like(x),
+                         ((x - top) / temperature).exp())
+    order = torch.sort(x, dim=-1, descending=True, stable=True)[1]
+    ranked = weight.gather(-1, order)
+    rank = torch.arange(x.shape[-1], device=x.device)
+    keep = (rank < top_k) | (top_k <= 0)
+    ranked = ranked * keep
+    before = ranked.cumsum(-1) - ranked
+    keep &= ((before <= top_p * ranked.sum(-1, keepdim=True))
+             | ~((top_p > 0) & (top_p < 1)))
+    keep &= ~(ranked < min_p.clamp(max=1.0))
+    kept = torch.zeros_like(keep).scatter(-1, order, keep)
+    upto = (weight * kept).cumsum(-1)
+    total = upto[:, -1:]
+    target = torch.minimum(uniform * total, total * (1 - 2.0 ** -53))
+    token = (upto <= target).sum(-1)
+    # uniform numbers outside 0..1 still fall on a kept token
+    index = torch.arange(x.shape[-1], device=x.device)
+    some = kept & (weight > 0)
+    last = torch.where(some, index, torch.full_like(index, -1)).amax(-1)
+    first = torch.where(some, index,
+                        torch.full_like(index, x.shape[-1])).amin(-1)
+    token = torch.maximum(torch.minimum(token, last), first)
+    void = x.isnan().any(-1) | (top[:, 0] == float("-inf"))
+    return torch.where(void, torch.full_like(token, -1), token)
