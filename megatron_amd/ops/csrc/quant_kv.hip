@@ -284,56 +284,455 @@ __global__ __launch_bounds__(256) void dequantize_kernel(
   }
 }
 
-// One wave per query row: lanes share the tokens for the scores, then the
-// values of a token for the output.
-template <typename T>
-__global__ __launch_bounds__(64) void attention_kernel(
-    CacheView cache, const T* __restrict__ q, long q_ss, long q_bs, long q_ns,
-    T* __restrict__ out, int n, Start start, float scale, long window,
-    long sinks) {
-  __shared__ float q_row[256];
-  const int lane = threadIdx.x, h = cache.h;
-  const int head = blockIdx.x, ib = blockIdx.y;
-  const long is = blockIdx.z;
-  const long bh = (long)ib * cache.heads + head / (n / cache.heads);
-  T* o = out + ((is * cache.b + ib) * n + head) * h;
-  const long t0 = start.of(ib), pos = t0 + is;
-  if (t0 < 0 || pos >= cache.capacity) {
-    for (int d = lane; d < h; d += 64)
-      o[d] = DTypeTraits<T>::from_float(t0 < 0 ? 0.f : NAN);
+// ---------------------------------------------------------------------------
+// Attention. A workgroup of four waves takes up to 16 MT query rows (heads of
+// one key head x new tokens) and a share of the tokens; each wave takes every
+// fourth tile of 32 tokens and keeps a running maximum, sum and output of its
+// own, joined through LDS at the end, and across workgroups by a second
+// kernel. Per tile, with g = lane / 16 and r = lane % 16:
+//
+//   S^T = K Q^T: the codes of token r and the head's quarter g come as one
+//       load, become fp16 in registers and are the A operand; S^T leaves the
+//       matrix core with query row r and tokens 4g + i in each lane.
+//   O^T += V^T P^T: that is just the layout of the B operand P^T, if the
+//       contraction runs over tokens in the order 4g + i of the tile's first
+//       half, then of its second; the cache holds values in that order. No
+//       value crosses lanes but in the rare update of the maximum.
+//
+// Codes become fp16 by or-ing them into 1024 + code, which is exact, and one
+// rounded multiply-add by the group's scale and zero point. Query rows are
+// brought to a maximum in [1, 2) by a power of two first, so that bf16 values
+// are exact in fp16 too. Sums and statistics are held in 32 bits, weights
+// rounded to fp16 (2^-12 each, against 2^-9 for bf16).
+
+using h2 = __attribute__((ext_vector_type(2))) _Float16;
+using h8 = __attribute__((ext_vector_type(8))) _Float16;
+using f4 = __attribute__((ext_vector_type(4))) float;
+
+constexpr int kTile = 32;       // tokens of a wave's step
+constexpr int kLeast = 128;     // tokens of a workgroup at least
+constexpr float kUnset = -3e38f;  // maximum before the first score
+constexpr float kSlack = 8.f;   // weights reach 2^8 before the maximum moves
+
+struct AttentionArgs {
+  CacheView cache;
+  const void* q;
+  long q_ss, q_bs, q_ns;
+  void* out;
+  float* part_o;   // [b * heads, chunks, rows, H], unless chunks == 1
+  float* part_ml;  // [b * heads, chunks, rows, 2]
+  int n, s, rep, rows, q_blocks, chunks;
+  float scale_log2e;
+  long window, sinks;
+  Start start;
+};
+
+// The tiles that some row of [first, last] sees: those of the sinks, then
+// those from the window's begin to the last row's position.
+struct Tiles {
+  long sink, low, count;
+  __device__ __forceinline__ long at(long i) const {
+    return i < sink ? i : low + i - sink;
+  }
+};
+
+__device__ __forceinline__ Tiles tiles_of(const AttentionArgs& a, long t0,
+                                          int first_row, int last_row) {
+  const long last = min(t0 + last_row / a.rep, a.cache.capacity - 1);
+  Tiles t{0, 0, 0};
+  const long end = last / kTile + 1;
+  if (a.window > 0) {
+    const long low = max(0l, t0 + first_row / a.rep - a.window + 1);
+    t.low = low / kTile;
+    t.sink = min((a.sinks + kTile - 1) / kTile, t.low);
+  }
+  t.count = t.sink + max(0l, end - t.low);
+  return t;
+}
+
+// tiles of one workgroup, a multiple of what four waves take at once
+__device__ __forceinline__ long chunk_tiles(long count, int chunks) {
+  const long per = (count + chunks - 1) / chunks;
+  return max((per + 3) / 4 * 4, (long)(kLeast / kTile));
+}
+
+template <int WORDS>
+__device__ __forceinline__ void load_words(unsigned (&w)[WORDS],
+                                           const void* p) {
+  if constexpr (WORDS == 1) {
+    w[0] = *(const unsigned*)p;
+  } else if constexpr (WORDS == 2) {
+    const uint2 v = *(const uint2*)p;
+    w[0] = v.x, w[1] = v.y;
+  } else {
+    for (int i = 0; i < WORDS; i += 4) {
+      const uint4 v = ((const uint4*)p)[i / 4];
+      w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
+    }
+  }
+}
+
+__device__ __forceinline__ h2 as_h2(unsigned u) {
+  return __builtin_bit_cast(h2, u);
+}
+
+// the four pairs of codes in a word, times scale plus zero point
+__device__ __forceinline__ void pairs_of(h2 (&y)[4], unsigned word, h2 scale,
+                                         h2 zero) {
+  const unsigned up = word >> 8;
+  const h2 big = {(_Float16)1024, (_Float16)1024};
+  const h2 part = {(_Float16)0.0625, (_Float16)0.0625};
+  const h2 less = {(_Float16)-64, (_Float16)-64};
+  const h2 x0 = as_h2((word & 0x000f000fu) | 0x64006400u) - big;
+  const h2 x1 = __builtin_elementwise_fma(
+      as_h2((word & 0x00f000f0u) | 0x64006400u), part, less);
+  const h2 x2 = as_h2((up & 0x000f000fu) | 0x64006400u) - big;
+  const h2 x3 = __builtin_elementwise_fma(
+      as_h2((up & 0x00f000f0u) | 0x64006400u), part, less);
+  y[0] = __builtin_elementwise_fma(x0, scale, zero);
+  y[1] = __builtin_elementwise_fma(x1, scale, zero);
+  y[2] = __builtin_elementwise_fma(x2, scale, zero);
+  y[3] = __builtin_elementwise_fma(x3, scale, zero);
+}
+
+__device__ __forceinline__ h8 join(h2 a, h2 b, h2 c, h2 d) {
+  return h8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+}
+
+template <int H>
+struct HeadShape {
+  static constexpr int kWords = H / 32;     // dwords of keys in a lane
+  static constexpr int kKeyGroups = H >= 256 ? H / 128 : 1;
+  static constexpr int kQuarters = H >= 64 ? H / 64 : 1;
+  static constexpr int kValueWords = 2 * kQuarters;  // for four tokens
+  static constexpr int kBlocks = H / 16;    // of 16 output values
+  static constexpr int kGroups = H / kGroup;
+};
+
+// what a lane holds of a tile: two halves of 16 tokens
+template <int H>
+struct TileRegs {
+  using S = HeadShape<H>;
+  unsigned k[2][S::kWords], km[2][S::kKeyGroups];
+  unsigned v[2][S::kValueWords], vm[2][4];
+};
+
+template <int H>
+__device__ __forceinline__ void load_tile(TileRegs<H>& t,
+                                          const unsigned char* k_codes,
+                                          const __half* k_meta,
+                                          const unsigned char* v_codes,
+                                          const __half* v_meta, long tile) {
+  using S = HeadShape<H>;
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  const unsigned char* kc = k_codes + tile * kTile * (H / 2);
+  const __half* km = k_meta + tile * kTile * S::kGroups * 2;
+  const unsigned char* vc = v_codes + tile * (kTile / 4) * 128 * S::kQuarters;
+  const __half* vm = v_meta + tile * (kTile / 4) * 8;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    load_words(t.k[half], kc + (half * 16 + r) * (H / 2) + g * (H / 8));
+    load_words(t.km[half], km + ((half * 16 + r) * S::kGroups +
+                                 g * (H / 4) / kGroup) * 2);
+    load_words(t.v[half], vc + ((half * 4 + g) * 16 + r) * 8 * S::kQuarters);
+    load_words(t.vm[half], vm + (half * 4 + g) * 8);
+  }
+}
+
+template <typename T, int H, int MT>
+__global__ __launch_bounds__(256) void attention_kernel(AttentionArgs a) {
+  using S = HeadShape<H>;
+  __shared__ h8 q_lds[MT][S::kWords][64];
+  __shared__ float c_lds[MT][16];
+  __shared__ float ml_lds[4][16][2];
+  __shared__ float o_lds[4][16][H + 1];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int r = lane & 15, g = lane >> 4;
+
+  // workgroups that share tokens are 8 apart: they run on the same die, whose
+  // second level cache holds the tokens between them
+  const int x = blockIdx.x & 7;
+  const int rest = blockIdx.x >> 3;
+  const int block = rest % a.q_blocks;
+  const long work = (long)(rest / a.q_blocks) * 8 + x;
+  const long pairs = (long)a.cache.b * a.cache.heads;
+  if (work >= pairs * a.chunks) return;
+  const int chunk = work % a.chunks;
+  const long bh = work / a.chunks;
+  const int ib = bh / a.cache.heads, kv_head = bh % a.cache.heads;
+  const int row0 = block * 16 * MT;
+  const int row1 = min(a.rows, row0 + 16 * MT) - 1;
+  const long t0 = a.start.of(ib);
+  const bool idle = t0 < 0 || t0 >= a.cache.capacity;
+  Tiles tiles{0, 0, 0};
+  if (!idle) tiles = tiles_of(a, t0, row0, row1);
+  const long per = chunk_tiles(tiles.count, a.chunks);
+  const long i_low = chunk * per;
+  const long i_high = min(tiles.count, i_low + per);
+  if (i_low >= i_high && a.chunks > 1) return;  // the join leaves it out
+
+  for (int mt = wave; mt < MT; mt += 4) {
+    const int row = row0 + mt * 16 + r;
+    float v[H / 4], peak = 0.f;
+    const bool real = row < a.rows;
+    const T* q = (const T*)a.q;
+    if (real)
+      q += (long)(row / a.rep) * a.q_ss + ib * a.q_bs +
+           (long)(kv_head * a.rep + row % a.rep) * a.q_ns + g * (H / 4);
+#pragma unroll
+    for (int i = 0; i < H / 4; ++i) {
+      v[i] = real ? DTypeTraits<T>::to_float(q[i]) : 0.f;
+      peak = fmaxf(peak, fabsf(v[i]));
+    }
+    peak = fmaxf(peak, __shfl_xor(peak, 16, WAVE_SIZE));
+    peak = fmaxf(peak, __shfl_xor(peak, 32, WAVE_SIZE));
+    const int e =
+        peak > 0.f && peak < INFINITY ? __builtin_amdgcn_frexp_expf(peak) - 1
+                                      : 0;
+#pragma unroll
+    for (int w = 0; w < S::kWords; ++w) {
+      h8 y;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        y[i] = (_Float16)__builtin_amdgcn_ldexpf(v[w * 8 + i], -e);
+      q_lds[mt][w][lane] = y;
+    }
+    if (g == 0) c_lds[mt][r] = __builtin_amdgcn_ldexpf(a.scale_log2e, e);
+  }
+  __syncthreads();
+
+  float c[MT], m[MT], l[MT];
+  long pos[MT];
+  f4 o[MT][S::kBlocks];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    c[mt] = c_lds[mt][r];
+    m[mt] = kUnset;
+    l[mt] = 0.f;
+    pos[mt] = t0 + (row0 + mt * 16 + r) / a.rep;
+#pragma unroll
+    for (int j = 0; j < S::kBlocks; ++j) o[mt][j] = f4{0.f, 0.f, 0.f, 0.f};
+  }
+  // whole tiles from here on need a look at each token's place
+  const long pos_first = t0 + row0 / a.rep, pos_last = t0 + row1 / a.rep;
+
+  const unsigned char* k_codes = a.cache.k_codes + bh * a.cache.room * (H / 2);
+  const __half* k_meta = a.cache.k_meta + bh * a.cache.room * S::kGroups * 2;
+  const unsigned char* v_codes =
+      a.cache.v_codes + bh * (a.cache.room / 4) * 128 * S::kQuarters;
+  const __half* v_meta = a.cache.v_meta +
+                         (bh * S::kGroups + r * S::kBlocks / kGroup) *
+                             (a.cache.room / 4) * 8;
+
+  TileRegs<H> next;
+  long i = i_low + wave;
+  if (i < i_high)
+    load_tile<H>(next, k_codes, k_meta, v_codes, v_meta, tiles.at(i));
+  for (; i < i_high; i += 4) {
+    const long tile = tiles.at(i);
+    const TileRegs<H> now = next;
+    if (i + 4 < i_high)
+      load_tile<H>(next, k_codes, k_meta, v_codes, v_meta, tiles.at(i + 4));
+
+    f4 st[MT][2];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) st[mt][half] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < S::kWords; ++w) {
+        const h2 sz =
+            as_h2(now.km[half][w * S::kKeyGroups / S::kWords]);
+        h2 y[4];
+        pairs_of(y, now.k[half][w], h2{sz.x, sz.x}, h2{sz.y, sz.y});
+        const h8 k8 = join(y[0], y[1], y[2], y[3]);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+          st[mt][half] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+              k8, q_lds[mt][w][lane], st[mt][half], 0, 0, 0);
+      }
+    }
+
+    const long t_tile = tile * kTile;
+    const bool partly =
+        t_tile + kTile - 1 > pos_first ||
+        (a.window > 0 && t_tile <= pos_last - a.window);
+    h8 p8[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      float sc[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sc[e] = st[mt][e >> 2][e & 3] * c[mt];
+      if (partly) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const long t = t_tile + (e >> 2) * 16 + g * 4 + (e & 3);
+          const bool seen =
+              t <= pos[mt] &&
+              (a.window <= 0 || t > pos[mt] - a.window || t < a.sinks);
+          sc[e] = seen ? sc[e] : -INFINITY;
+        }
+      }
+      float peak = sc[0];
+#pragma unroll
+      for (int e = 1; e < 8; ++e) peak = fmaxf(peak, sc[e]);
+      if (__any(peak > m[mt] + kSlack)) {
+        peak = fmaxf(peak, __shfl_xor(peak, 16, WAVE_SIZE));
+        peak = fmaxf(peak, __shfl_xor(peak, 32, WAVE_SIZE));
+        const float up = fmaxf(m[mt], peak);
+        const float alpha = __builtin_amdgcn_exp2f(m[mt] - up);
+        m[mt] = up;
+        l[mt] *= alpha;
+#pragma unroll
+        for (int j = 0; j < S::kBlocks; ++j) o[mt][j] *= alpha;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float w = __builtin_amdgcn_exp2f(sc[e] - m[mt]);
+        l[mt] += w;
+        p8[mt][e] = (_Float16)w;
+      }
+    }
+
+    // a NaN group's scale is taken as 0: what sees the token is NaN already
+    h2 vs[2][2], vz[2][2];
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        vs[half][p] = __builtin_elementwise_max(as_h2(now.vm[half][p]),
+                                                h2{0, 0});
+        vz[half][p] = as_h2(now.vm[half][2 + p]);
+      }
+#pragma unroll
+    for (int quarter = 0; quarter < S::kQuarters; ++quarter) {
+      h2 y[2][2][4];
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+          pairs_of(y[half][p], now.v[half][p * S::kQuarters + quarter],
+                   vs[half][p], vz[half][p]);
+#pragma unroll
+      for (int j = 0; j < (H >= 64 ? 4 : 2); ++j) {
+        const h8 v8 = join(y[0][0][j], y[0][1][j], y[1][0][j], y[1][1][j]);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+          o[mt][quarter * 4 + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+              v8, p8[mt], o[mt][quarter * 4 + j], 0, 0, 0);
+      }
+    }
+  }
+
+  // join the four waves
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    float sum = l[mt] + __shfl_xor(l[mt], 16, WAVE_SIZE);
+    sum += __shfl_xor(sum, 32, WAVE_SIZE);
+    if (mt) __syncthreads();
+    if (g == 0) {
+      ml_lds[wave][r][0] = m[mt];
+      ml_lds[wave][r][1] = sum;
+    }
+    __syncthreads();
+    float top = kUnset;
+    for (int w = 0; w < 4; ++w) top = fmaxf(top, ml_lds[w][r][0]);
+    const float f = __builtin_amdgcn_exp2f(m[mt] - top);
+#pragma unroll
+    for (int j = 0; j < S::kBlocks; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        o_lds[wave][r][(4 * g + e) * S::kBlocks + j] = o[mt][j][e] * f;
+    __syncthreads();
+    for (int idx = threadIdx.x; idx < 16 * H; idx += 256) {
+      const int rr = idx / H, d = idx % H;
+      const int row = row0 + mt * 16 + rr;
+      if (row >= a.rows) break;
+      float y = 0.f, sum = 0.f, high = kUnset;
+      for (int w = 0; w < 4; ++w) {
+        y += o_lds[w][rr][d];
+        high = fmaxf(high, ml_lds[w][rr][0]);
+      }
+      for (int w = 0; w < 4; ++w)
+        sum += ml_lds[w][rr][1] * __builtin_amdgcn_exp2f(ml_lds[w][rr][0] -
+                                                         high);
+      if (a.chunks > 1) {
+        const long at = (bh * a.chunks + chunk) * a.rows + row;
+        a.part_o[at * H + d] = y;
+        if (d == 0) {
+          a.part_ml[at * 2] = high;
+          a.part_ml[at * 2 + 1] = sum;
+        }
+      } else {
+        const long i = row / a.rep;
+        const int head = kv_head * a.rep + row % a.rep;
+        float z = y / sum;
+        if (t0 < 0) z = 0.f;
+        else if (t0 + i >= a.cache.capacity) z = NAN;
+        T* out = (T*)a.out + ((i * a.cache.b + ib) * a.n + head) * H + d;
+        *out = DTypeTraits<T>::from_float(z);
+      }
+    }
+  }
+}
+
+// Joins the chunks of a row: one workgroup per (row, key head, sequence).
+template <typename T, int H, int MT>
+__global__ __launch_bounds__(256) void join_kernel(AttentionArgs a) {
+  constexpr int kSide = 256 / H;  // chunks read side by side
+  __shared__ float o_lds[kSide][H], l_lds[kSide];
+  const long bh = blockIdx.x / a.rows;
+  const int row = blockIdx.x % a.rows;
+  const int ib = bh / a.cache.heads, kv_head = bh % a.cache.heads;
+  const int d = threadIdx.x % H, side = threadIdx.x / H;
+  const long t0 = a.start.of(ib);
+  const long i = row / a.rep;
+  const int head = kv_head * a.rep + row % a.rep;
+  T* out = (T*)a.out + ((i * a.cache.b + ib) * a.n + head) * H;
+  if (t0 < 0 || t0 + i >= a.cache.capacity) {
+    if (side == 0) out[d] = DTypeTraits<T>::from_float(t0 < 0 ? 0.f : NAN);
     return;
   }
-  const T* qx = q + is * q_ss + ib * q_bs + head * q_ns;
-  for (int d = lane; d < h; d += 64)
-    q_row[d] = DTypeTraits<T>::to_float(qx[d]) * scale;
-  __syncthreads();
-  float m = -INFINITY, sum = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-  for (long base = 0; base <= pos; base += 64) {
-    const long t = base + lane;
-    const bool seen = t <= pos &&
-                      (window <= 0 || t > pos - window || t < sinks);
-    float score = -INFINITY;
-    if (seen) {
-      score = 0.f;
-      for (int d = 0; d < h; ++d) score += q_row[d] * held_k(cache, bh, t, d);
-    }
-    if (!__any(seen)) continue;
-    const bool broken = __any(score != score);
-    const float peak = broken ? NAN : fmaxf(m, wave_reduce_max(score));
-    const float alpha = m == -INFINITY ? 0.f : __expf(m - peak);
-    const float p = seen ? __expf(score - peak) : 0.f;
-    m = peak;
-    sum = sum * alpha + wave_reduce_sum(p);
-    for (int i = 0; i < 4; ++i) acc[i] *= alpha;
-    for (int j = 0; j < 64; ++j) {
-      const float pj = __shfl(p, j, WAVE_SIZE);
-      if (!__shfl((int)seen, j, WAVE_SIZE)) continue;
-      for (int i = 0; i < 4 && lane + 64 * i < h; ++i)
-        acc[i] += pj * held_v(cache, bh, base + j, lane + 64 * i);
-    }
+  const int row0 = row / (16 * MT) * 16 * MT;
+  const Tiles tiles =
+      tiles_of(a, t0, row0, min(a.rows, row0 + 16 * MT) - 1);
+  const long per = chunk_tiles(tiles.count, a.chunks);
+  const int used = (tiles.count + per - 1) / per;
+  const long at = bh * a.chunks * a.rows + row;
+  float top = kUnset;
+  for (int c = 0; c < used; ++c)
+    top = fmaxf(top, a.part_ml[(at + (long)c * a.rows) * 2]);
+  float y = 0.f, sum = 0.f;
+  for (int c = side; c < used; c += kSide) {
+    const long from = at + (long)c * a.rows;
+    const float f = __builtin_amdgcn_exp2f(a.part_ml[from * 2] - top);
+    sum += a.part_ml[from * 2 + 1] * f;
+    y += a.part_o[from * H + d] * f;
   }
-  for (int i = 0; i < 4 && lane + 64 * i < h; ++i)
-    o[lane + 64 * i] = DTypeTraits<T>::from_float(acc[i] / sum);
+  o_lds[side][d] = y;
+  if (d == 0) l_lds[side] = sum;
+  __syncthreads();
+  if (side == 0) {
+    for (int w = 1; w < kSide; ++w) {
+      y += o_lds[w][d];
+      sum += l_lds[w];
+    }
+    out[d] = DTypeTraits<T>::from_float(y / sum);
+  }
+}
+
+template <typename T, int H, int MT>
+void launch_attention(AttentionArgs a, hipStream_t stream) {
+  const long work = (long)a.cache.b * a.cache.heads * a.chunks;
+  const long grid = (work + 7) / 8 * 8 * a.q_blocks;
+  const long joins = (long)a.cache.b * a.cache.heads * a.rows;
+  TORCH_CHECK(grid < (1l << 31) && joins < (1l << 31),
+              "quant_kv: too many queries at once");
+  hipLaunchKernelGGL((attention_kernel<T, H, MT>), dim3(grid), dim3(256), 0,
+                     stream, a);
+  if (a.chunks > 1)
+    hipLaunchKernelGGL((join_kernel<T, H, MT>), dim3(joins), dim3(256), 0,
+                       stream, a);
 }
 
 CacheView view_of(const std::vector<torch::Tensor>& c, int64_t capacity) {
@@ -505,14 +904,61 @@ torch::Tensor quant_kv_attention(std::vector<torch::Tensor> buffers,
   const Start at = start_of(start, start_s, cache, buffers[0]);
   auto out = torch::empty({s, cache.b, (long)n * cache.h}, query.options());
   if (out.numel() == 0) return out;
+  AttentionArgs a;
+  a.cache = cache;
+  a.q = query.data_ptr();
+  a.q_ss = query.stride(0);
+  a.q_bs = query.stride(1);
+  a.q_ns = query.stride(2);
+  a.out = out.data_ptr();
+  a.n = n;
+  a.s = (int)s;
+  a.rep = n / cache.heads;
+  TORCH_CHECK(s * a.rep < (1l << 30), "quant_kv: too many queries at once");
+  a.rows = (int)s * a.rep;
+  a.scale_log2e = (float)(scale * 1.4426950408889634);
+  a.window = window;
+  a.sinks = sinks;
+  a.start = at;
+
+  // query tiles of a workgroup: one decodes, more share the work on the codes
+  const int tiles = (a.rows + 15) / 16;
+  const int mt = tiles == 1 ? 1 : tiles == 2 || cache.h == 256 ? 2 : 4;
+  a.q_blocks = (tiles + mt - 1) / mt;
+  // enough workgroups to fill the card; each has 128 tokens at least. Where
+  // a sequence ends is on the device, so the shares are settled there.
+  const long span =
+      window > 0 ? std::min<long>(cache.capacity, window + sinks + s)
+                 : cache.capacity;
+  const long base = (long)cache.b * cache.heads * a.q_blocks;
+  const long most = (span + kLeast - 1) / kLeast;
+  a.chunks = (int)std::max<long>(
+      1, std::min<long>(std::min<long>(most, 256), (2048 + base - 1) / base));
+  torch::Tensor part;
+  a.part_o = a.part_ml = nullptr;
+  if (a.chunks > 1) {
+    const long parts = (long)cache.b * cache.heads * a.chunks * a.rows;
+    part = torch::empty({parts * (cache.h + 2)},
+                        query.options().dtype(torch::kFloat32));
+    a.part_o = part.data_ptr<float>();
+    a.part_ml = a.part_o + parts * cache.h;
+  }
   auto stream = c10::hip::getCurrentHIPStream();
-  TORCH_CHECK(s < 65536 && cache.b < 65536);
-  dim3 grid(n, cache.b, s);
 #define LAUNCH_ATTENTION(T)                                                  \
-  hipLaunchKernelGGL((attention_kernel<T>), grid, dim3(64), 0, stream,       \
-                     cache, (const T*)query.data_ptr(), query.stride(0),     \
-                     query.stride(1), query.stride(2), (T*)out.data_ptr(),   \
-                     n, at, (float)scale, (long)window, (long)sinks)
+  switch (cache.h * 8 + mt) {                                                \
+    case 32 * 8 + 1: launch_attention<T, 32, 1>(a, stream); break;           \
+    case 32 * 8 + 2: launch_attention<T, 32, 2>(a, stream); break;           \
+    case 32 * 8 + 4: launch_attention<T, 32, 4>(a, stream); break;           \
+    case 64 * 8 + 1: launch_attention<T, 64, 1>(a, stream); break;           \
+    case 64 * 8 + 2: launch_attention<T, 64, 2>(a, stream); break;           \
+    case 64 * 8 + 4: launch_attention<T, 64, 4>(a, stream); break;           \
+    case 128 * 8 + 1: launch_attention<T, 128, 1>(a, stream); break;         \
+    case 128 * 8 + 2: launch_attention<T, 128, 2>(a, stream); break;         \
+    case 128 * 8 + 4: launch_attention<T, 128, 4>(a, stream); break;         \
+    case 256 * 8 + 1: launch_attention<T, 256, 1>(a, stream); break;         \
+    case 256 * 8 + 2: launch_attention<T, 256, 2>(a, stream); break;         \
+    default: TORCH_CHECK(false, "quant_kv: head_dim");                       \
+  }
   DISPATCH_HALF(query, LAUNCH_ATTENTION);
 #undef LAUNCH_ATTENTION
   HIP_CHECK(hipGetLastError());
