@@ -302,8 +302,12 @@ __global__ __launch_bounds__(256) void dequantize_kernel(
 // Codes become fp16 by or-ing them into 1024 + code, which is exact, and one
 // rounded multiply-add by the group's scale and zero point. Query rows are
 // brought to a maximum in [1, 2) by a power of two first, so that bf16 values
-// are exact in fp16 too. Sums and statistics are held in 32 bits, weights
-// rounded to fp16 (2^-12 each, against 2^-9 for bf16).
+// are exact in fp16 too. Sums and statistics are held in 32 bits. The operands
+// are rounded to fp16, a relative 2^-11 at most, under the 2^-8 of a bf16
+// output. That of an fp16 output is 2^-11 too, so there (EXACT) what the
+// roundings left out is multiplied as well, and the middle of each group,
+// z + 8 s, goes through products of its own in two parts: the output is as far
+// off as the plain form's (2.1e-4) against 4.4e-4 without.
 
 using h2 = __attribute__((ext_vector_type(2))) _Float16;
 using h8 = __attribute__((ext_vector_type(8))) _Float16;
@@ -376,23 +380,32 @@ __device__ __forceinline__ h2 as_h2(unsigned u) {
   return __builtin_bit_cast(h2, u);
 }
 
-// the four pairs of codes in a word, times scale plus zero point
-__device__ __forceinline__ void pairs_of(h2 (&y)[4], unsigned word, h2 scale,
-                                         h2 zero) {
+// The four pairs of codes in a word as values scale * code + zero; with EXACT
+// as scale * (code - 8), which takes 15 bits: rounded, and what that left out.
+template <bool EXACT>
+__device__ __forceinline__ void pairs_of(h2 (&y)[4], h2 (&left)[4],
+                                         unsigned word, h2 scale, h2 zero) {
   const unsigned up = word >> 8;
-  const h2 big = {(_Float16)1024, (_Float16)1024};
+  constexpr float kOff = EXACT ? 8.f : 0.f;
+  const h2 big = {(_Float16)(1024 + kOff), (_Float16)(1024 + kOff)};
   const h2 part = {(_Float16)0.0625, (_Float16)0.0625};
-  const h2 less = {(_Float16)-64, (_Float16)-64};
-  const h2 x0 = as_h2((word & 0x000f000fu) | 0x64006400u) - big;
-  const h2 x1 = __builtin_elementwise_fma(
-      as_h2((word & 0x00f000f0u) | 0x64006400u), part, less);
-  const h2 x2 = as_h2((up & 0x000f000fu) | 0x64006400u) - big;
-  const h2 x3 = __builtin_elementwise_fma(
-      as_h2((up & 0x00f000f0u) | 0x64006400u), part, less);
-  y[0] = __builtin_elementwise_fma(x0, scale, zero);
-  y[1] = __builtin_elementwise_fma(x1, scale, zero);
-  y[2] = __builtin_elementwise_fma(x2, scale, zero);
-  y[3] = __builtin_elementwise_fma(x3, scale, zero);
+  const h2 less = {(_Float16)(-64 - kOff), (_Float16)(-64 - kOff)};
+  const h2 x[4] = {
+      as_h2((word & 0x000f000fu) | 0x64006400u) - big,
+      __builtin_elementwise_fma(as_h2((word & 0x00f000f0u) | 0x64006400u),
+                                part, less),
+      as_h2((up & 0x000f000fu) | 0x64006400u) - big,
+      __builtin_elementwise_fma(as_h2((up & 0x00f000f0u) | 0x64006400u), part,
+                                less)};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if constexpr (EXACT) {
+      y[j] = x[j] * scale;
+      left[j] = __builtin_elementwise_fma(x[j], scale, -y[j]);
+    } else {
+      y[j] = __builtin_elementwise_fma(x[j], scale, zero);
+    }
+  }
 }
 
 __device__ __forceinline__ h8 join(h2 a, h2 b, h2 c, h2 d) {
@@ -442,7 +455,9 @@ __device__ __forceinline__ void load_tile(TileRegs<H>& t,
 template <typename T, int H, int MT>
 __global__ __launch_bounds__(256) void attention_kernel(AttentionArgs a) {
   using S = HeadShape<H>;
+  constexpr bool kExact = std::is_same_v<T, __half>;
   __shared__ h8 q_lds[MT][S::kWords][64];
+  __shared__ h8 sum_lds[kExact ? MT : 1][64];  // of q, in two parts
   __shared__ float c_lds[MT][16];
   __shared__ float ml_lds[4][16][2];
   __shared__ float o_lds[4][16][H + 1];
@@ -489,13 +504,26 @@ __global__ __launch_bounds__(256) void attention_kernel(AttentionArgs a) {
     const int e =
         peak > 0.f && peak < INFINITY ? __builtin_amdgcn_frexp_expf(peak) - 1
                                       : 0;
+    float sum[S::kKeyGroups] = {};
 #pragma unroll
     for (int w = 0; w < S::kWords; ++w) {
       h8 y;
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+      for (int i = 0; i < 8; ++i) {
         y[i] = (_Float16)__builtin_amdgcn_ldexpf(v[w * 8 + i], -e);
+        sum[w * S::kKeyGroups / S::kWords] += (float)y[i];
+      }
       q_lds[mt][w][lane] = y;
+    }
+    if constexpr (kExact) {
+      h8 y = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < S::kKeyGroups; ++i) {
+        const _Float16 high = (_Float16)sum[i];
+        y[3 * i] = y[3 * i + 1] = high;
+        y[3 * i + 2] = (_Float16)(sum[i] - (float)high);
+      }
+      sum_lds[mt][lane] = y;
     }
     if (g == 0) c_lds[mt][r] = __builtin_amdgcn_ldexpf(a.scale_log2e, e);
   }
@@ -503,12 +531,13 @@ __global__ __launch_bounds__(256) void attention_kernel(AttentionArgs a) {
 
   float c[MT], m[MT], l[MT];
   long pos[MT];
-  f4 o[MT][S::kBlocks];
+  f4 o[MT][S::kBlocks], mid[MT];  // mid: the groups' middles' part
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
     c[mt] = c_lds[mt][r];
     m[mt] = kUnset;
     l[mt] = 0.f;
+    mid[mt] = f4{0.f, 0.f, 0.f, 0.f};
     pos[mt] = t0 + (row0 + mt * 16 + r) / a.rep;
 #pragma unroll
     for (int j = 0; j < S::kBlocks; ++j) o[mt][j] = f4{0.f, 0.f, 0.f, 0.f};
@@ -539,17 +568,39 @@ __global__ __launch_bounds__(256) void attention_kernel(AttentionArgs a) {
     for (int half = 0; half < 2; ++half) {
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) st[mt][half] = f4{0.f, 0.f, 0.f, 0.f};
+      if constexpr (kExact) {
+        h8 c8 = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < S::kKeyGroups; ++i) {
+          const h2 sz = as_h2(now.km[half][i]);
+          const float middle = fmaf(8.f, (float)sz.x, (float)sz.y);
+          c8[3 * i] = c8[3 * i + 2] = (_Float16)middle;
+          c8[3 * i + 1] = (_Float16)(middle - (float)c8[3 * i]);
+        }
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+          st[mt][half] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+              c8, sum_lds[mt][lane], st[mt][half], 0, 0, 0);
+      }
 #pragma unroll
       for (int w = 0; w < S::kWords; ++w) {
         const h2 sz =
             as_h2(now.km[half][w * S::kKeyGroups / S::kWords]);
-        h2 y[4];
-        pairs_of(y, now.k[half][w], h2{sz.x, sz.x}, h2{sz.y, sz.y});
+        h2 y[4], z[4];
+        pairs_of<kExact>(y, z, now.k[half][w], h2{sz.x, sz.x},
+                         h2{sz.y, sz.y});
         const h8 k8 = join(y[0], y[1], y[2], y[3]);
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
           st[mt][half] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
               k8, q_lds[mt][w][lane], st[mt][half], 0, 0, 0);
+        if constexpr (kExact) {
+          const h8 l8 = join(z[0], z[1], z[2], z[3]);
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+            st[mt][half] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                l8, q_lds[mt][w][lane], st[mt][half], 0, 0, 0);
+        }
       }
     }
 
@@ -557,7 +608,7 @@ __global__ __launch_bounds__(256) void attention_kernel(AttentionArgs a) {
     const bool partly =
         t_tile + kTile - 1 > pos_first ||
         (a.window > 0 && t_tile <= pos_last - a.window);
-    h8 p8[MT];
+    h8 p8[MT], p_left[MT];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       float sc[8];
@@ -585,12 +636,15 @@ __global__ __launch_bounds__(256) void attention_kernel(AttentionArgs a) {
         l[mt] *= alpha;
 #pragma unroll
         for (int j = 0; j < S::kBlocks; ++j) o[mt][j] *= alpha;
+        if constexpr (kExact) mid[mt] *= alpha;
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float w = __builtin_amdgcn_exp2f(sc[e] - m[mt]);
         l[mt] += w;
         p8[mt][e] = (_Float16)w;
+        if constexpr (kExact)
+          p_left[mt][e] = (_Float16)(w - (float)p8[mt][e]);
       }
     }
 
@@ -604,15 +658,36 @@ __global__ __launch_bounds__(256) void attention_kernel(AttentionArgs a) {
                                                 h2{0, 0});
         vz[half][p] = as_h2(now.vm[half][2 + p]);
       }
+    if constexpr (kExact) {
+      h8 high, low;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float middle =
+            fmaf(8.f, (float)vs[e >> 2][(e >> 1) & 1][e & 1],
+                 (float)vz[e >> 2][(e >> 1) & 1][e & 1]);
+        high[e] = (_Float16)middle;
+        low[e] = (_Float16)(middle - (float)high[e]);
+      }
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        mid[mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(high, p8[mt],
+                                                         mid[mt], 0, 0, 0);
+        mid[mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(high, p_left[mt],
+                                                         mid[mt], 0, 0, 0);
+        mid[mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(low, p8[mt],
+                                                         mid[mt], 0, 0, 0);
+      }
+    }
 #pragma unroll
     for (int quarter = 0; quarter < S::kQuarters; ++quarter) {
-      h2 y[2][2][4];
+      h2 y[2][2][4], z[2][2][4];
 #pragma unroll
       for (int half = 0; half < 2; ++half)
 #pragma unroll
         for (int p = 0; p < 2; ++p)
-          pairs_of(y[half][p], now.v[half][p * S::kQuarters + quarter],
-                   vs[half][p], vz[half][p]);
+          pairs_of<kExact>(y[half][p], z[half][p],
+                           now.v[half][p * S::kQuarters + quarter],
+                           vs[half][p], vz[half][p]);
 #pragma unroll
       for (int j = 0; j < (H >= 64 ? 4 : 2); ++j) {
         const h8 v8 = join(y[0][0][j], y[0][1][j], y[1][0][j], y[1][1][j]);
@@ -620,6 +695,17 @@ __global__ __launch_bounds__(256) void attention_kernel(AttentionArgs a) {
         for (int mt = 0; mt < MT; ++mt)
           o[mt][quarter * 4 + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
               v8, p8[mt], o[mt][quarter * 4 + j], 0, 0, 0);
+        if constexpr (kExact) {
+          const h8 l8 =
+              join(z[0][0][j], z[0][1][j], z[1][0][j], z[1][1][j]);
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            o[mt][quarter * 4 + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                v8, p_left[mt], o[mt][quarter * 4 + j], 0, 0, 0);
+            o[mt][quarter * 4 + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                l8, p8[mt], o[mt][quarter * 4 + j], 0, 0, 0);
+          }
+        }
       }
     }
   }
@@ -642,7 +728,8 @@ __global__ __launch_bounds__(256) void attention_kernel(AttentionArgs a) {
     for (int j = 0; j < S::kBlocks; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        o_lds[wave][r][(4 * g + e) * S::kBlocks + j] = o[mt][j][e] * f;
+        o_lds[wave][r][(4 * g + e) * S::kBlocks + j] =
+            (o[mt][j][e] + mid[mt][e]) * f;
     __syncthreads();
     for (int idx = threadIdx.x; idx < 16 * H; idx += 256) {
       const int rr = idx / H, d = idx % H;
