@@ -384,18 +384,19 @@ __device__ __forceinline__ h2 as_h2(unsigned u) {
 // as scale * (code - 8), which takes 15 bits: rounded, and what that left out.
 template <bool EXACT>
 __device__ __forceinline__ void pairs_of(h2 (&y)[4], h2 (&left)[4],
-                                         unsigned word, h2 scale, h2 zero) {
-  const unsigned up = word >> 8;
+                                         unsigned word, h2 scale, h2 zero,
+                                         unsigned exponent) {
+  const unsigned up = word >> 8, e = exponent;
   constexpr float kOff = EXACT ? 8.f : 0.f;
   const h2 big = {(_Float16)(1024 + kOff), (_Float16)(1024 + kOff)};
   const h2 part = {(_Float16)0.0625, (_Float16)0.0625};
   const h2 less = {(_Float16)(-64 - kOff), (_Float16)(-64 - kOff)};
   const h2 x[4] = {
-      as_h2((word & 0x000f000fu) | 0x64006400u) - big,
-      __builtin_elementwise_fma(as_h2((word & 0x00f000f0u) | 0x64006400u),
+      as_h2((word & 0x000f000fu) | e) - big,
+      __builtin_elementwise_fma(as_h2((word & 0x00f000f0u) | e),
                                 part, less),
-      as_h2((up & 0x000f000fu) | 0x64006400u) - big,
-      __builtin_elementwise_fma(as_h2((up & 0x00f000f0u) | 0x64006400u), part,
+      as_h2((up & 0x000f000fu) | e) - big,
+      __builtin_elementwise_fma(as_h2((up & 0x00f000f0u) | e), part,
                                 less)};
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -430,38 +431,110 @@ struct TileRegs {
   unsigned v[2][S::kValueWords], vm[2][4];
 };
 
+// A tile in LDS: its keys' codes, its values' codes, its keys' scales, its
+// values' scales, each as in memory. It comes straight from memory, so that
+// tiles in flight take no registers.
 template <int H>
-__device__ __forceinline__ void load_tile(TileRegs<H>& t,
-                                          const unsigned char* k_codes,
-                                          const __half* k_meta,
-                                          const unsigned char* v_codes,
-                                          const __half* v_meta, long tile) {
+struct TileLds {
   using S = HeadShape<H>;
-  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-  const unsigned char* kc = k_codes + tile * kTile * (H / 2);
-  const __half* km = k_meta + tile * kTile * S::kGroups * 2;
-  const unsigned char* vc = v_codes + tile * (kTile / 4) * 128 * S::kQuarters;
-  const __half* vm = v_meta + tile * (kTile / 4) * 8;
+  static constexpr int kV = kTile * H / 2;
+  static constexpr int kKm = kV + 1024 * S::kQuarters;
+  static constexpr int kVm = kKm + 128 * S::kGroups;
+  static constexpr int kBytes = kVm + 128 * S::kGroups;
+  static constexpr int kLoads = (kTile * H / 2 + 1023) / 1024 +
+                                S::kQuarters + (S::kGroups > 4 ? 2 : 1);
+};
+
+// 16 bytes a lane from memory to LDS at `to` + 16 lane. Not known to the
+// compiler as a load: wait_loads() is what orders it.
+__device__ __forceinline__ void load_to_lds(unsigned to, const void* from) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %1, off"
+      :
+      : "s"(to), "v"(from)
+      : "memory", "m0");
+}
+
+template <int LEFT>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" : : "n"(LEFT) : "memory");
+}
+
+struct HeadMemory {
+  const unsigned char *k_codes, *v_codes;
+  const __half *k_meta, *v_meta;
+  long meta_stride;  // from group to group of v_meta
+};
+
+template <int H>
+__device__ __forceinline__ void fetch_tile(unsigned to, const HeadMemory& m,
+                                           long tile, int lane) {
+  using S = HeadShape<H>;
+  using L = TileLds<H>;
+  const unsigned char* k = m.k_codes + tile * kTile * (H / 2) + lane * 16;
+  const unsigned char* v =
+      m.v_codes + tile * (kTile / 4) * 128 * S::kQuarters + lane * 16;
+  const __half* km = m.k_meta + tile * kTile * S::kGroups * 2;
+  const __half* vm = m.v_meta + tile * (kTile / 4) * 8;
+  if (H >= 64 || lane < 32)
+#pragma unroll
+    for (int i = 0; i < (kTile * H / 2 + 1023) / 1024; ++i)
+      load_to_lds(to + i * 1024, k + i * 1024);
+#pragma unroll
+  for (int i = 0; i < S::kQuarters; ++i)
+    load_to_lds(to + L::kV + i * 1024, v + i * 1024);
+  constexpr int kLanes = 8 * S::kGroups;  // 16 bytes each
+  const int j = lane - (kLanes < 64 ? kLanes : 0);
+  const __half* vm_lane = vm + (j >> 3) * m.meta_stride + (j & 7) * 8;
+  if constexpr (kLanes < 64) {  // both kinds of scales in one load
+    if (lane < 2 * kLanes)
+      load_to_lds(to + L::kKm, lane < kLanes ? km + lane * 8 : vm_lane);
+  } else {
+    load_to_lds(to + L::kKm, km + lane * 8);
+    load_to_lds(to + L::kVm, vm_lane);
+  }
+}
+
+template <int H>
+__device__ __forceinline__ void read_tile(TileRegs<H>& t,
+                                          const unsigned char* from,
+                                          int lane) {
+  using S = HeadShape<H>;
+  using L = TileLds<H>;
+  const int r = lane & 15, g = lane >> 4;
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
-    load_words(t.k[half], kc + (half * 16 + r) * (H / 2) + g * (H / 8));
-    load_words(t.km[half], km + ((half * 16 + r) * S::kGroups +
-                                 g * (H / 4) / kGroup) * 2);
-    load_words(t.v[half], vc + ((half * 4 + g) * 16 + r) * 8 * S::kQuarters);
-    load_words(t.vm[half], vm + (half * 4 + g) * 8);
+    load_words(t.k[half], from + (half * 16 + r) * (H / 2) + g * (H / 8));
+    load_words(t.km[half],
+               from + L::kKm + ((half * 16 + r) * S::kGroups +
+                                g * (H / 4) / kGroup) * 4);
+    load_words(t.v[half], from + L::kV +
+                              ((half * 4 + g) * 16 + r) * 8 * S::kQuarters);
+    load_words(t.vm[half], from + L::kVm +
+                               ((r * S::kBlocks / kGroup) * 8 + half * 4 + g) *
+                                   16);
   }
 }
 
 template <typename T, int H, int MT>
-__global__ __launch_bounds__(256) void attention_kernel(AttentionArgs a) {
+__global__ __launch_bounds__(256, MT * H <= 128 ? 3 : MT * H <= 256 ? 2 : 1)
+void attention_kernel(AttentionArgs a) {
   using S = HeadShape<H>;
+  using L = TileLds<H>;
+  constexpr int kAhead = 2;  // tiles in flight or in use, per wave
   constexpr bool kExact = std::is_same_v<T, __half>;
   __shared__ h8 q_lds[MT][S::kWords][64];
   __shared__ h8 sum_lds[kExact ? MT : 1][64];  // of q, in two parts
   __shared__ float c_lds[MT][16];
   __shared__ float ml_lds[4][16][2];
-  __shared__ float o_lds[4][16][H + 1];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  // the waves' tiles, and once those are used up their outputs
+  constexpr int kRing = 4 * kAhead * L::kBytes, kOut = 4 * 16 * (H + 1) * 4;
+  __shared__ __align__(16) unsigned char ring[kRing > kOut ? kRing : kOut];
+  float(*o_lds)[16][H + 1] = (float(*)[16][H + 1])ring;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, g = lane >> 4;
 
   // workgroups that share tokens are 8 apart: they run on the same die, whose
@@ -545,23 +618,45 @@ __global__ __launch_bounds__(256) void attention_kernel(AttentionArgs a) {
   // whole tiles from here on need a look at each token's place
   const long pos_first = t0 + row0 / a.rep, pos_last = t0 + row1 / a.rep;
 
-  const unsigned char* k_codes = a.cache.k_codes + bh * a.cache.room * (H / 2);
-  const __half* k_meta = a.cache.k_meta + bh * a.cache.room * S::kGroups * 2;
-  const unsigned char* v_codes =
-      a.cache.v_codes + bh * (a.cache.room / 4) * 128 * S::kQuarters;
-  const __half* v_meta = a.cache.v_meta +
-                         (bh * S::kGroups + r * S::kBlocks / kGroup) *
-                             (a.cache.room / 4) * 8;
+  const HeadMemory memory{
+      a.cache.k_codes + bh * a.cache.room * (H / 2),
+      a.cache.v_codes + bh * (a.cache.room / 4) * 128 * S::kQuarters,
+      a.cache.k_meta + bh * a.cache.room * S::kGroups * 2,
+      a.cache.v_meta + bh * a.cache.room * S::kGroups * 2,
+      a.cache.room * 2};
+  const unsigned char* mine = ring + wave * kAhead * L::kBytes;
+  const unsigned mine_at =
+      (unsigned)(unsigned long)(__attribute__((address_space(3)))
+                                const unsigned char*)mine;
+  unsigned exponent = 0x64006400u;  // in a register: and + or in one step
+  asm("" : "+v"(exponent));
+  h8 q_reg[S::kWords];
+  if constexpr (MT == 1)
+#pragma unroll
+    for (int w = 0; w < S::kWords; ++w) q_reg[w] = q_lds[0][w][lane];
+  auto q_of = [&](int mt, int w) {
+    return MT == 1 ? q_reg[w] : q_lds[mt][w][lane];
+  };
 
-  TileRegs<H> next;
   long i = i_low + wave;
-  if (i < i_high)
-    load_tile<H>(next, k_codes, k_meta, v_codes, v_meta, tiles.at(i));
-  for (; i < i_high; i += 4) {
+#pragma unroll
+  for (int ahead = 0; ahead < kAhead; ++ahead)
+    if (i + 4 * ahead < i_high)
+      fetch_tile<H>(mine_at + ahead * L::kBytes, memory,
+                    tiles.at(i + 4 * ahead), lane);
+  for (int slot = 0; i < i_high;
+       i += 4, slot = slot + 1 == kAhead ? 0 : slot + 1) {
     const long tile = tiles.at(i);
-    const TileRegs<H> now = next;
-    if (i + 4 < i_high)
-      load_tile<H>(next, k_codes, k_meta, v_codes, v_meta, tiles.at(i + 4));
+    if (i + 4 * (kAhead - 1) < i_high)
+      wait_loads<(kAhead - 1) * L::kLoads>();
+    else
+      wait_loads<0>();
+    TileRegs<H> now;
+    read_tile<H>(now, mine + slot * L::kBytes, lane);
+    asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+    if (i + 4 * kAhead < i_high)
+      fetch_tile<H>(mine_at + slot * L::kBytes, memory,
+                    tiles.at(i + 4 * kAhead), lane);
 
     f4 st[MT][2];
 #pragma unroll
@@ -588,18 +683,18 @@ __global__ __launch_bounds__(256) void attention_kernel(AttentionArgs a) {
             as_h2(now.km[half][w * S::kKeyGroups / S::kWords]);
         h2 y[4], z[4];
         pairs_of<kExact>(y, z, now.k[half][w], h2{sz.x, sz.x},
-                         h2{sz.y, sz.y});
+                         h2{sz.y, sz.y}, exponent);
         const h8 k8 = join(y[0], y[1], y[2], y[3]);
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
           st[mt][half] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-              k8, q_lds[mt][w][lane], st[mt][half], 0, 0, 0);
+              k8, q_of(mt, w), st[mt][half], 0, 0, 0);
         if constexpr (kExact) {
           const h8 l8 = join(z[0], z[1], z[2], z[3]);
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt)
             st[mt][half] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                l8, q_lds[mt][w][lane], st[mt][half], 0, 0, 0);
+                l8, q_of(mt, w), st[mt][half], 0, 0, 0);
         }
       }
     }
@@ -687,7 +782,7 @@ __global__ __launch_bounds__(256) void attention_kernel(AttentionArgs a) {
         for (int p = 0; p < 2; ++p)
           pairs_of<kExact>(y[half][p], z[half][p],
                            now.v[half][p * S::kQuarters + quarter],
-                           vs[half][p], vz[half][p]);
+                           vs[half][p], vz[half][p], exponent);
 #pragma unroll
       for (int j = 0; j < (H >= 64 ? 4 : 2); ++j) {
         const h8 v8 = join(y[0][0][j], y[0][1][j], y[1][0][j], y[1][1][j]);
@@ -711,6 +806,7 @@ __global__ __launch_bounds__(256) void attention_kernel(AttentionArgs a) {
   }
 
   // join the four waves
+  __syncthreads();
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
     float sum = l[mt] + __shfl_xor(l[mt], 16, WAVE_SIZE);
