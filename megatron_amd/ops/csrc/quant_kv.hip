@@ -325,39 +325,62 @@ struct AttentionArgs {
   void* out;
   float* part_o;   // [b * heads, chunks, rows, H], unless chunks == 1
   float* part_ml;  // [b * heads, chunks, rows, 2]
-  int n, s, rep, rows, q_blocks, chunks;
+  int n, s, rep, rows, q_blocks, chunks, share;
   float scale_log2e;
   long window, sinks;
   Start start;
+  bool q_wide;  // rows of q lie at multiples of 16 bytes
 };
 
-// The tiles that some row of [first, last] sees: those of the sinks, then
-// those from the window's begin to the last row's position.
+// The tiles that some row of [first, last] of a sequence sees: those of the
+// sinks, then those from the window's begin to the last row's position.
 struct Tiles {
-  long sink, low, count;
-  __device__ __forceinline__ long at(long i) const {
+  int sink, low, count;
+  __device__ __forceinline__ int at(int i) const {
     return i < sink ? i : low + i - sink;
   }
 };
 
 __device__ __forceinline__ Tiles tiles_of(const AttentionArgs& a, long t0,
                                           int first_row, int last_row) {
-  const long last = min(t0 + last_row / a.rep, a.cache.capacity - 1);
   Tiles t{0, 0, 0};
-  const long end = last / kTile + 1;
+  if (t0 < 0 || t0 >= a.cache.capacity) return t;
+  const int last = (int)min(t0 + (unsigned)last_row / (unsigned)a.rep,
+                            a.cache.capacity - 1);
   if (a.window > 0) {
-    const long low = max(0l, t0 + first_row / a.rep - a.window + 1);
-    t.low = low / kTile;
-    t.sink = min((a.sinks + kTile - 1) / kTile, t.low);
+    const long low =
+        max(0l, t0 + (unsigned)first_row / (unsigned)a.rep - a.window + 1);
+    t.low = (int)(low / kTile);
+    t.sink = (int)min((a.sinks + kTile - 1) / kTile, (long)t.low);
   }
-  t.count = t.sink + max(0l, end - t.low);
+  t.count = t.sink + max(0, last / kTile + 1 - t.low);
   return t;
 }
 
-// tiles of one workgroup, a multiple of what four waves take at once
-__device__ __forceinline__ long chunk_tiles(long count, int chunks) {
-  const long per = (count + chunks - 1) / chunks;
-  return max((per + 3) / 4 * 4, (long)(kLeast / kTile));
+// Tiles of a workgroup: what all sequences have, shared out over `share`
+// workgroups, so that sequences of any lengths end together; a multiple of
+// what four waves take at once, and enough for the grid to reach the end.
+// Every lane of a wave calls this; all get the same.
+__device__ __forceinline__ int chunk_tiles(const AttentionArgs& a,
+                                           const Tiles& own, int first_row,
+                                           int last_row) {
+  const int lane = threadIdx.x & 63;
+  int total = 0;
+  if (a.start.stride == 0) {
+    total = own.count * a.cache.b;
+  } else {
+    for (int ib = lane; ib < a.cache.b; ib += 64)
+      total += tiles_of(a, a.start.of(ib), first_row, last_row).count;
+    for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o, WAVE_SIZE);
+  }
+  const unsigned even =
+      ((unsigned)total * (unsigned)a.cache.heads + a.share - 1) /
+      (unsigned)a.share;
+  const unsigned least =
+      ((unsigned)own.count + a.chunks - 1) / (unsigned)a.chunks;
+  const int per = (int)max(even, least);
+  return __builtin_amdgcn_readfirstlane(
+      max((per + 3) & ~3, kLeast / kTile));
 }
 
 template <int WORDS>
@@ -539,39 +562,71 @@ void attention_kernel(AttentionArgs a) {
 
   // workgroups that share tokens are 8 apart: they run on the same die, whose
   // second level cache holds the tokens between them
-  const int x = blockIdx.x & 7;
-  const int rest = blockIdx.x >> 3;
-  const int block = rest % a.q_blocks;
-  const long work = (long)(rest / a.q_blocks) * 8 + x;
-  const long pairs = (long)a.cache.b * a.cache.heads;
+  const unsigned x = blockIdx.x & 7, rest = blockIdx.x >> 3;
+  const int block = rest % (unsigned)a.q_blocks;
+  const unsigned work = rest / (unsigned)a.q_blocks * 8 + x;
+  const unsigned pairs = a.cache.b * a.cache.heads;
   if (work >= pairs * a.chunks) return;
-  const int chunk = work % a.chunks;
-  const long bh = work / a.chunks;
-  const int ib = bh / a.cache.heads, kv_head = bh % a.cache.heads;
+  // the first shares of all sequences come first, those that may be empty last
+  const int chunk = work / pairs;
+  const long bh = work % pairs;
+  const int ib = (unsigned)bh / (unsigned)a.cache.heads;
+  const int kv_head = (unsigned)bh % (unsigned)a.cache.heads;
   const int row0 = block * 16 * MT;
   const int row1 = min(a.rows, row0 + 16 * MT) - 1;
   const long t0 = a.start.of(ib);
-  const bool idle = t0 < 0 || t0 >= a.cache.capacity;
-  Tiles tiles{0, 0, 0};
-  if (!idle) tiles = tiles_of(a, t0, row0, row1);
-  const long per = chunk_tiles(tiles.count, a.chunks);
-  const long i_low = chunk * per;
-  const long i_high = min(tiles.count, i_low + per);
+  const Tiles tiles = tiles_of(a, t0, row0, row1);
+  const int per = a.chunks > 1 ? chunk_tiles(a, tiles, row0, row1)
+                               : tiles.count;
+  const int i_low = chunk * per;
+  const int i_high = min(tiles.count, i_low + per);
   if (i_low >= i_high && a.chunks > 1) return;  // the join leaves it out
+
+  const HeadMemory memory{
+      a.cache.k_codes + bh * a.cache.room * (H / 2),
+      a.cache.v_codes + bh * (a.cache.room / 4) * 128 * S::kQuarters,
+      a.cache.k_meta + bh * a.cache.room * S::kGroups * 2,
+      a.cache.v_meta + bh * a.cache.room * S::kGroups * 2,
+      a.cache.room * 2};
+  const unsigned char* mine = ring + wave * kAhead * L::kBytes;
+  const unsigned mine_at =
+      (unsigned)(unsigned long)(__attribute__((address_space(3)))
+                                const unsigned char*)mine;
+  int i = i_low + wave;
+#pragma unroll
+  for (int ahead = 0; ahead < kAhead; ++ahead)
+    if (i + 4 * ahead < i_high)
+      fetch_tile<H>(mine_at + ahead * L::kBytes, memory,
+                    tiles.at(i + 4 * ahead), lane);
 
   for (int mt = wave; mt < MT; mt += 4) {
     const int row = row0 + mt * 16 + r;
     float v[H / 4], peak = 0.f;
     const bool real = row < a.rows;
+    const unsigned token = (unsigned)row / (unsigned)a.rep;
     const T* q = (const T*)a.q;
     if (real)
-      q += (long)(row / a.rep) * a.q_ss + ib * a.q_bs +
-           (long)(kv_head * a.rep + row % a.rep) * a.q_ns + g * (H / 4);
+      q += (long)token * a.q_ss + ib * a.q_bs +
+           (long)(kv_head * a.rep + row - token * a.rep) * a.q_ns +
+           g * (H / 4);
+    if (a.q_wide) {
 #pragma unroll
-    for (int i = 0; i < H / 4; ++i) {
-      v[i] = real ? DTypeTraits<T>::to_float(q[i]) : 0.f;
-      peak = fmaxf(peak, fabsf(v[i]));
+      for (int i = 0; i < H / 4; i += 8) {
+        union {
+          uint4 u;
+          T t[8];
+        } y;
+        y.u = real ? *(const uint4*)(q + i) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[i + e] = DTypeTraits<T>::to_float(y.t[e]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < H / 4; ++i)
+        v[i] = real ? DTypeTraits<T>::to_float(q[i]) : 0.f;
     }
+#pragma unroll
+    for (int i = 0; i < H / 4; ++i) peak = fmaxf(peak, fabsf(v[i]));
     peak = fmaxf(peak, __shfl_xor(peak, 16, WAVE_SIZE));
     peak = fmaxf(peak, __shfl_xor(peak, 32, WAVE_SIZE));
     const int e =
@@ -618,16 +673,6 @@ void attention_kernel(AttentionArgs a) {
   // whole tiles from here on need a look at each token's place
   const long pos_first = t0 + row0 / a.rep, pos_last = t0 + row1 / a.rep;
 
-  const HeadMemory memory{
-      a.cache.k_codes + bh * a.cache.room * (H / 2),
-      a.cache.v_codes + bh * (a.cache.room / 4) * 128 * S::kQuarters,
-      a.cache.k_meta + bh * a.cache.room * S::kGroups * 2,
-      a.cache.v_meta + bh * a.cache.room * S::kGroups * 2,
-      a.cache.room * 2};
-  const unsigned char* mine = ring + wave * kAhead * L::kBytes;
-  const unsigned mine_at =
-      (unsigned)(unsigned long)(__attribute__((address_space(3)))
-                                const unsigned char*)mine;
   unsigned exponent = 0x64006400u;  // in a register: and + or in one step
   asm("" : "+v"(exponent));
   h8 q_reg[S::kWords];
@@ -638,15 +683,9 @@ void attention_kernel(AttentionArgs a) {
     return MT == 1 ? q_reg[w] : q_lds[mt][w][lane];
   };
 
-  long i = i_low + wave;
-#pragma unroll
-  for (int ahead = 0; ahead < kAhead; ++ahead)
-    if (i + 4 * ahead < i_high)
-      fetch_tile<H>(mine_at + ahead * L::kBytes, memory,
-                    tiles.at(i + 4 * ahead), lane);
   for (int slot = 0; i < i_high;
        i += 4, slot = slot + 1 == kAhead ? 0 : slot + 1) {
-    const long tile = tiles.at(i);
+    const int tile = tiles.at(i);
     if (i + 4 * (kAhead - 1) < i_high)
       wait_loads<(kAhead - 1) * L::kLoads>();
     else
@@ -699,7 +738,7 @@ void attention_kernel(AttentionArgs a) {
       }
     }
 
-    const long t_tile = tile * kTile;
+    const long t_tile = (long)tile * kTile;
     const bool partly =
         t_tile + kTile - 1 > pos_first ||
         (a.window > 0 && t_tile <= pos_last - a.window);
@@ -859,48 +898,60 @@ void attention_kernel(AttentionArgs a) {
   }
 }
 
-// Joins the chunks of a row: one workgroup per (row, key head, sequence).
+// Joins the chunks of a row: one workgroup per (row, key head, sequence), a
+// wave for every fourth chunk, each lane with H / 64 values.
 template <typename T, int H, int MT>
 __global__ __launch_bounds__(256) void join_kernel(AttentionArgs a) {
-  constexpr int kSide = 256 / H;  // chunks read side by side
-  __shared__ float o_lds[kSide][H], l_lds[kSide];
-  const long bh = blockIdx.x / a.rows;
-  const int row = blockIdx.x % a.rows;
-  const int ib = bh / a.cache.heads, kv_head = bh % a.cache.heads;
-  const int d = threadIdx.x % H, side = threadIdx.x / H;
+  constexpr int kEach = H >= 64 ? H / 64 : 1;
+  __shared__ float o_lds[4][H], l_lds[4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const unsigned bh = blockIdx.x / (unsigned)a.rows;
+  const unsigned row = blockIdx.x - bh * a.rows;
+  const unsigned ib = bh / (unsigned)a.cache.heads;
+  const unsigned kv_head = bh - ib * a.cache.heads;
+  const int d = lane * kEach;
   const long t0 = a.start.of(ib);
-  const long i = row / a.rep;
-  const int head = kv_head * a.rep + row % a.rep;
-  T* out = (T*)a.out + ((i * a.cache.b + ib) * a.n + head) * H;
+  const unsigned i = row / (unsigned)a.rep;
+  const int head = kv_head * a.rep + row - i * a.rep;
+  T* out = (T*)a.out + (((long)i * a.cache.b + ib) * a.n + head) * H;
   if (t0 < 0 || t0 + i >= a.cache.capacity) {
-    if (side == 0) out[d] = DTypeTraits<T>::from_float(t0 < 0 ? 0.f : NAN);
+    if (wave == 0 && d < H)
+      for (int e = 0; e < kEach; ++e)
+        out[d + e] = DTypeTraits<T>::from_float(t0 < 0 ? 0.f : NAN);
     return;
   }
   const int row0 = row / (16 * MT) * 16 * MT;
-  const Tiles tiles =
-      tiles_of(a, t0, row0, min(a.rows, row0 + 16 * MT) - 1);
-  const long per = chunk_tiles(tiles.count, a.chunks);
+  const int row1 = min(a.rows, row0 + 16 * MT) - 1;
+  const Tiles tiles = tiles_of(a, t0, row0, row1);
+  const unsigned per = chunk_tiles(a, tiles, row0, row1);
   const int used = (tiles.count + per - 1) / per;
-  const long at = bh * a.chunks * a.rows + row;
+  // from chunk to chunk of a (sequence, key head, row)
+  const long step = a.rows;
+  const float* ml = a.part_ml + ((long)bh * a.chunks * step + row) * 2;
+  const float* po = a.part_o + ((long)bh * a.chunks * step + row) * H + d;
   float top = kUnset;
-  for (int c = 0; c < used; ++c)
-    top = fmaxf(top, a.part_ml[(at + (long)c * a.rows) * 2]);
-  float y = 0.f, sum = 0.f;
-  for (int c = side; c < used; c += kSide) {
-    const long from = at + (long)c * a.rows;
-    const float f = __builtin_amdgcn_exp2f(a.part_ml[from * 2] - top);
-    sum += a.part_ml[from * 2 + 1] * f;
-    y += a.part_o[from * H + d] * f;
+  for (int c = lane; c < used; c += 64) top = fmaxf(top, ml[c * step * 2]);
+  top = wave_reduce_max(top);
+  float y[kEach] = {}, sum = 0.f;
+#pragma unroll 4
+  for (int c = wave; c < used; c += 4) {
+    const float2 ml_c = *(const float2*)(ml + c * step * 2);
+    float x[kEach] = {};
+    if (d < H)
+      for (int e = 0; e < kEach; ++e) x[e] = po[c * step * H + e];
+    const float f = __builtin_amdgcn_exp2f(ml_c.x - top);
+    sum += ml_c.y * f;
+    for (int e = 0; e < kEach; ++e) y[e] += x[e] * f;
   }
-  o_lds[side][d] = y;
-  if (d == 0) l_lds[side] = sum;
+  if (d < H)
+    for (int e = 0; e < kEach; ++e) o_lds[wave][d + e] = y[e];
+  if (lane == 0) l_lds[wave] = sum;
   __syncthreads();
-  if (side == 0) {
-    for (int w = 1; w < kSide; ++w) {
-      y += o_lds[w][d];
-      sum += l_lds[w];
-    }
-    out[d] = DTypeTraits<T>::from_float(y / sum);
+  if (threadIdx.x < H) {
+    const int t = threadIdx.x;
+    out[t] = DTypeTraits<T>::from_float(
+        (o_lds[0][t] + o_lds[1][t] + o_lds[2][t] + o_lds[3][t]) /
+        (l_lds[0] + l_lds[1] + l_lds[2] + l_lds[3]));
   }
 }
 
@@ -1108,15 +1159,25 @@ torch::Tensor quant_kv_attention(std::vector<torch::Tensor> buffers,
   const int tiles = (a.rows + 15) / 16;
   const int mt = tiles == 1 ? 1 : tiles == 2 || cache.h == 256 ? 2 : 4;
   a.q_blocks = (tiles + mt - 1) / mt;
-  // enough workgroups to fill the card; each has 128 tokens at least. Where
-  // a sequence ends is on the device, so the shares are settled there.
+  a.q_wide = cache.h >= 32 && (unsigned long)a.q % 16 == 0 &&
+             a.q_ss % 8 == 0 && a.q_bs % 8 == 0 && a.q_ns % 8 == 0;
+  // Workgroups that the card holds at once share the tokens. Where sequences
+  // end is on the device, so the shares are settled there; the grid has room
+  // for a sequence of several times the mean length.
   const long span =
-      window > 0 ? std::min<long>(cache.capacity, window + sinks + s)
+      window > 0 ? std::min<long>(cache.capacity, window + sinks + s + 64)
                  : cache.capacity;
   const long base = (long)cache.b * cache.heads * a.q_blocks;
+  const int resident = mt * cache.h <= 128 ? 3 : mt * cache.h <= 256 ? 2 : 1;
+  const long slots = 256 * resident;
+  const long aim = base < slots / 2 ? slots - base / 2 : 2 * slots;
   const long most = (span + kLeast - 1) / kLeast;
   a.chunks = (int)std::max<long>(
-      1, std::min<long>(std::min<long>(most, 256), (2048 + base - 1) / base));
+      1, std::min<long>(std::min<long>(most, 256),
+                        (4 * aim + base - 1) / base));
+  a.share = (int)std::max<long>(1, aim / a.q_blocks);
+  TORCH_CHECK(cache.capacity < (1l << 31) && base * a.chunks < (1l << 31),
+              "quant_kv: too many tokens or queries at once");
   torch::Tensor part;
   a.part_o = a.part_ml = nullptr;
   if (a.chunks > 1) {
