@@ -325,7 +325,8 @@ struct AttentionArgs {
   void* out;
   float* part_o;   // [b * heads, chunks, rows, H], unless chunks == 1
   float* part_ml;  // [b * heads, chunks, rows, 2]
-  int n, s, rep, rows, q_blocks, chunks, share;
+  int n, s, rep, rows, q_blocks, chunks, groups;
+  int* part_per;  // tiles of a chunk
   float scale_log2e;
   long window, sinks;
   Start start;
@@ -357,30 +358,76 @@ __device__ __forceinline__ Tiles tiles_of(const AttentionArgs& a, long t0,
   return t;
 }
 
-// Tiles of a workgroup: what all sequences have, shared out over `share`
-// workgroups, so that sequences of any lengths end together; a multiple of
-// what four waves take at once, and enough for the grid to reach the end.
-// Every lane of a wave calls this; all get the same.
-__device__ __forceinline__ int chunk_tiles(const AttentionArgs& a,
-                                           const Tiles& own, int first_row,
-                                           int last_row) {
+// Sums over the wave by row shifts and broadcasts: lane i gets that of the
+// lanes up to i.
+__device__ __forceinline__ int wave_scan(int v) {
+#define SCAN_STEP(CTRL, ROWS) \
+  v += __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false)
+  SCAN_STEP(0x111, 0xf);  // from 1, 2, 4, 8 lanes below, within 16
+  SCAN_STEP(0x112, 0xf);
+  SCAN_STEP(0x114, 0xf);
+  SCAN_STEP(0x118, 0xf);
+  SCAN_STEP(0x142, 0xa);  // from the last lane of the 16 below
+  SCAN_STEP(0x143, 0xc);  // from lane 31
+#undef SCAN_STEP
+  return v;
+}
+
+__device__ __forceinline__ int wave_total(int v) {
+  return __builtin_amdgcn_readlane(wave_scan(v), 63);
+}
+
+// A workgroup's share of the tokens, settled from where the sequences end:
+// each share has `per` tiles, a multiple of what four waves take at once, and
+// `per` is about the least with which the shares of all sequences are no more
+// than `groups`. They are numbered without gaps: workgroups that end at once
+// between others would leave some of the card's engines with more than they
+// hold and others idle, since they are dealt out in turn.
+struct Share {
+  int per, ib, chunk;  // ib < 0: none
+};
+
+__device__ __forceinline__ Share share_of(const AttentionArgs& a, int index) {
   const int lane = threadIdx.x & 63;
-  int total = 0;
-  if (a.start.stride == 0) {
-    total = own.count * a.cache.b;
-  } else {
-    for (int ib = lane; ib < a.cache.b; ib += 64)
-      total += tiles_of(a, a.start.of(ib), first_row, last_row).count;
-    for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o, WAVE_SIZE);
+  auto tiles_in = [&](int ib) {
+    return ib < a.cache.b ? tiles_of(a, a.start.of(ib), 0, a.rows - 1).count
+                          : 0;
+  };
+  const int first = tiles_in(lane);
+  auto total_of = [&](auto f) {
+    int t = f(first);
+    for (int ib = lane + 64; ib < a.cache.b; ib += 64) t += f(tiles_in(ib));
+    return wave_total(t);
+  };
+  int longest = first;
+  for (int ib = lane + 64; ib < a.cache.b; ib += 64)
+    longest = max(longest, tiles_in(ib));
+  for (int o = 32; o > 0; o >>= 1)
+    longest = max(longest, __shfl_xor(longest, o, WAVE_SIZE));
+  const int total = total_of([](int n) { return n; });
+  int per = max(kLeast / kTile, max((total + a.groups - 1) / a.groups,
+                                    (longest + a.chunks - 1) / a.chunks));
+  per = (per + 3) & ~3;
+  auto shares = [&](int n) {
+    return (int)(((unsigned)n + per - 1) / (unsigned)per);
+  };
+  // there are at least twice as many groups as sequences, so this ends
+  while (total_of(shares) > a.groups) per += max(4, per / 8 & ~3);
+  Share s{per, -1, 0};
+  int before = 0;
+  for (int low = 0; low < a.cache.b; low += 64) {
+    const int own = shares(low ? tiles_in(low + lane) : first);
+    const int upto = before + wave_scan(own);
+    const unsigned long after = __ballot(upto > index);
+    if (after) {
+      const int at = __builtin_ctzl(after);
+      s.ib = low + at;
+      s.chunk = index - __builtin_amdgcn_readlane(upto - own, at);
+      break;
+    }
+    before = __builtin_amdgcn_readlane(upto, 63);
   }
-  const unsigned even =
-      ((unsigned)total * (unsigned)a.cache.heads + a.share - 1) /
-      (unsigned)a.share;
-  const unsigned least =
-      ((unsigned)own.count + a.chunks - 1) / (unsigned)a.chunks;
-  const int per = (int)max(even, least);
-  return __builtin_amdgcn_readfirstlane(
-      max((per + 3) & ~3, kLeast / kTile));
+  return s;
 }
 
 template <int WORDS>
@@ -565,21 +612,25 @@ void attention_kernel(AttentionArgs a) {
   const unsigned x = blockIdx.x & 7, rest = blockIdx.x >> 3;
   const int block = rest % (unsigned)a.q_blocks;
   const unsigned work = rest / (unsigned)a.q_blocks * 8 + x;
-  const unsigned pairs = a.cache.b * a.cache.heads;
-  if (work >= pairs * a.chunks) return;
-  // the first shares of all sequences come first, those that may be empty last
-  const int chunk = work / pairs;
-  const long bh = work % pairs;
-  const int ib = (unsigned)bh / (unsigned)a.cache.heads;
-  const int kv_head = (unsigned)bh % (unsigned)a.cache.heads;
+  const unsigned index = work / (unsigned)a.cache.heads;
+  const int kv_head = work % (unsigned)a.cache.heads;
+  Share share{0, (int)index, 0};
+  if (a.chunks > 1) {
+    share = share_of(a, index);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *a.part_per = share.per;
+    if (share.ib < 0) return;
+  } else if (index >= (unsigned)a.cache.b) {
+    return;
+  }
+  const int ib = share.ib, chunk = share.chunk;
+  const long bh = (long)ib * a.cache.heads + kv_head;
   const int row0 = block * 16 * MT;
   const int row1 = min(a.rows, row0 + 16 * MT) - 1;
   const long t0 = a.start.of(ib);
   const Tiles tiles = tiles_of(a, t0, row0, row1);
-  const int per = a.chunks > 1 ? chunk_tiles(a, tiles, row0, row1)
-                               : tiles.count;
-  const int i_low = chunk * per;
-  const int i_high = min(tiles.count, i_low + per);
+  const int i_low = chunk * share.per;
+  const int i_high =
+      a.chunks > 1 ? min(tiles.count, i_low + share.per) : tiles.count;
   if (i_low >= i_high && a.chunks > 1) return;  // the join leaves it out
 
   const HeadMemory memory{
@@ -923,7 +974,7 @@ __global__ __launch_bounds__(256) void join_kernel(AttentionArgs a) {
   const int row0 = row / (16 * MT) * 16 * MT;
   const int row1 = min(a.rows, row0 + 16 * MT) - 1;
   const Tiles tiles = tiles_of(a, t0, row0, row1);
-  const unsigned per = chunk_tiles(a, tiles, row0, row1);
+  const unsigned per = *a.part_per;
   const int used = (tiles.count + per - 1) / per;
   // from chunk to chunk of a (sequence, key head, row)
   const long step = a.rows;
@@ -957,7 +1008,8 @@ __global__ __launch_bounds__(256) void join_kernel(AttentionArgs a) {
 
 template <typename T, int H, int MT>
 void launch_attention(AttentionArgs a, hipStream_t stream) {
-  const long work = (long)a.cache.b * a.cache.heads * a.chunks;
+  const long work =
+      (long)(a.chunks > 1 ? a.groups : a.cache.b) * a.cache.heads;
   const long grid = (work + 7) / 8 * 8 * a.q_blocks;
   const long joins = (long)a.cache.b * a.cache.heads * a.rows;
   TORCH_CHECK(grid < (1l << 31) && joins < (1l << 31),
@@ -1161,31 +1213,32 @@ torch::Tensor quant_kv_attention(std::vector<torch::Tensor> buffers,
   a.q_blocks = (tiles + mt - 1) / mt;
   a.q_wide = cache.h >= 32 && (unsigned long)a.q % 16 == 0 &&
              a.q_ss % 8 == 0 && a.q_bs % 8 == 0 && a.q_ns % 8 == 0;
-  // Workgroups that the card holds at once share the tokens. Where sequences
-  // end is on the device, so the shares are settled there; the grid has room
-  // for a sequence of several times the mean length.
+  // Workgroups that the card holds at once share the tokens, or, where there
+  // are about as many key heads and query blocks, one more for each of those.
+  // A sequence may be several times the mean in length.
   const long span =
       window > 0 ? std::min<long>(cache.capacity, window + sinks + s + 64)
                  : cache.capacity;
-  const long base = (long)cache.b * cache.heads * a.q_blocks;
+  const long each = (long)cache.heads * a.q_blocks, base = cache.b * each;
   const int resident = mt * cache.h <= 128 ? 3 : mt * cache.h <= 256 ? 2 : 1;
-  const long slots = 256 * resident;
-  const long aim = base < slots / 2 ? slots - base / 2 : 2 * slots;
+  a.groups = (int)std::max<long>(2l * cache.b, 256 * resident / each);
   const long most = (span + kLeast - 1) / kLeast;
   a.chunks = (int)std::max<long>(
       1, std::min<long>(std::min<long>(most, 256),
-                        (4 * aim + base - 1) / base));
-  a.share = (int)std::max<long>(1, aim / a.q_blocks);
-  TORCH_CHECK(cache.capacity < (1l << 31) && base * a.chunks < (1l << 31),
+                        4 * (a.groups * each + base - 1) / base));
+  TORCH_CHECK(cache.capacity < (1l << 31) && base * a.chunks < (1l << 31) &&
+                  a.groups * each < (1l << 31),
               "quant_kv: too many tokens or queries at once");
   torch::Tensor part;
   a.part_o = a.part_ml = nullptr;
+  a.part_per = nullptr;
   if (a.chunks > 1) {
     const long parts = (long)cache.b * cache.heads * a.chunks * a.rows;
-    part = torch::empty({parts * (cache.h + 2)},
+    part = torch::empty({parts * (cache.h + 2) + 1},
                         query.options().dtype(torch::kFloat32));
     a.part_o = part.data_ptr<float>();
     a.part_ml = a.part_o + parts * cache.h;
+    a.part_per = (int*)(a.part_ml + parts * 2);
   }
   auto stream = c10::hip::getCurrentHIPStream();
 #define LAUNCH_ATTENTION(T)                                                  \
