@@ -48,24 +48,46 @@ __device__ __forceinline__ unsigned order_key(float x) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-template <typename V>
-__device__ __forceinline__ V block_sum(V v, V* lds) {
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, WAVE_SIZE);
+__device__ __forceinline__ float key_value(unsigned key) {
+  return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+}
+
+constexpr int kBins = 2048;
+constexpr int kList = 256;  // candidates that are ranked one against another
+
+struct Lds {
+  u64 mass[kBins];
+  unsigned count[kBins];
+  u64 list_weight[kList];
+  unsigned list_key[kList];
+  u64 wave[2][kWaves];
+  double power[64];  // 2^(j / 64)
+  u64 answer[4];
+  unsigned listed, low, high;
+};
+
+template <typename V, typename F>
+__device__ __forceinline__ V block_reduce(V v, u64* lds, F join) {
+  for (int o = 32; o > 0; o >>= 1) v = join(v, __shfl_xor(v, o, WAVE_SIZE));
   __syncthreads();
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
   __syncthreads();
-  V total = 0;
-  for (int w = 0; w < kWaves; ++w) total += lds[w];
-  return total;
+  V all = (V)lds[0];
+  for (int w = 1; w < kWaves; ++w) all = join(all, (V)lds[w]);
+  return all;
+}
+
+template <typename V>
+__device__ __forceinline__ V block_sum(V v, u64* lds) {
+  return block_reduce(v, lds, [](V a, V b) { return a + b; });
 }
 
 // sum of the values of all threads before this one
-template <typename V>
-__device__ __forceinline__ V block_scan(V v, V* lds) {
+__device__ __forceinline__ u64 block_scan(u64 v, u64* lds) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  V up = v;
+  u64 up = v;
   for (int o = 1; o < 64; o <<= 1) {
-    const V other = __shfl_up(up, o, WAVE_SIZE);
+    const u64 other = __shfl_up(up, o, WAVE_SIZE);
     if (lane >= o) up += other;
   }
   __syncthreads();
@@ -80,133 +102,381 @@ __device__ __forceinline__ u64 floor_u64(double x, u64 most) {
   return x >= (double)most ? most : (u64)x;
 }
 
+// A row, read 16 bytes at a time where they lie within it. Each wave has a
+// run of indices of its own, so that sums by wave are sums in order.
+template <typename T>
+struct Row {
+  static constexpr int kVec = 16 / sizeof(T);
+  static constexpr int kBatch = 4;  // loads in flight
+  const T* x;
+  int vocab, shift;  // x - shift is a multiple of 16 bytes
+  int first, last;   // this wave's run
+
+  __device__ Row(const T* x, int vocab) : x(x), vocab(vocab) {
+    shift = (int)((unsigned long)x & 15) / (int)sizeof(T);
+    const int step = WAVE_SIZE * kVec;
+    const int run = ((vocab + shift + kWaves - 1) / kWaves + step - 1) /
+                    step * step;
+    const int wave = threadIdx.x >> 6;
+    first = min(vocab, max(0, wave * run - shift));
+    last = min(vocab, (wave + 1) * run - shift);
+  }
+
+  __device__ __forceinline__ float at(int i) const {
+    return DTypeTraits<T>::to_float(x[i]);
+  }
+
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
+    const int lane = threadIdx.x & 63;
+    // the run's begin lies on 16 bytes, but for the row's own
+    const int begin = first == 0 ? -shift : first;
+    for (int base = begin; base < last; base += kBatch * WAVE_SIZE * kVec) {
+      union {
+        uint4 u;
+        T t[kVec];
+      } v[kBatch];
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const int i = base + (k * WAVE_SIZE + lane) * kVec;
+        if (i >= 0 && i + kVec <= last) {
+          v[k].u = *(const uint4*)(x + i);
+        } else {
+#pragma unroll
+          for (int e = 0; e < kVec; ++e)
+            if (i + e >= 0 && i + e < last) v[k].t[e] = x[i + e];
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const int i = base + (k * WAVE_SIZE + lane) * kVec;
+#pragma unroll
+        for (int e = 0; e < kVec; ++e)
+          if (i + e >= 0 && i + e < last)
+            f(DTypeTraits<T>::to_float(v[k].t[e]));
+      }
+    }
+  }
+};
+
+// Weights of a row: 2^y with y = (x - top) / T log2 e <= 0, from a table of
+// 2^(j / 64) and a polynomial of the fourth degree on the rest, which is at
+// most ln 2 / 128 (relative error under 2^-44).
+struct Weights {
+  float top;
+  double per;  // log2 e / T, 64 times
+  int shift;
+  const double* power;
+
+  __device__ __forceinline__ double of(float v) const {
+    if (v == top) return 1.0;
+    const double y = fmax(((double)v - (double)top) * per, -64.0 * 1000.0);
+    const double k = rint(y);
+    const double r = (y - k) * (0.6931471805599453 / 64);
+    double p = fma(r, 1.0 / 24, 1.0 / 6);
+    p = fma(r, p, 0.5);
+    p = fma(r, p, 1.0);
+    p = fma(r, p, 1.0);
+    const int n = (int)k;
+    return ldexp(p * power[n & 63], n >> 6);
+  }
+  __device__ __forceinline__ u64 whole(double w) const {
+    const double high = trunc(ldexp(w, shift - 32));
+    const unsigned h = (unsigned)high;
+    return (u64)h << 32 | (unsigned)ldexp(ldexp(w, shift - 32) - high, 32);
+  }
+  __device__ __forceinline__ u64 whole_of(float v) const {
+    return whole(of(v));
+  }
+};
+
+// Tokens with a larger key are kept, and the first `ties` of those with this.
+struct Cut {
+  unsigned key;
+  u64 ties;
+};
+
+// Down from the largest key, where `limit` is passed: by count (MASS false)
+// the key of the limit-th token, by mass the least key whose larger ones weigh
+// at most `limit`. Tokens above `floor` count, which more than `limit` have;
+// low..high are their extreme keys, both finite.
+//
+// Each step shares the keys' range out over bins, finds the bin in which the
+// limit is passed and goes on within it, until it is one key or few tokens.
+template <bool MASS, typename T>
+__device__ Cut find_cut(Lds& lds, const Row<T>& row, const Weights& weights,
+                        unsigned low, unsigned high, u64 limit) {
+  const int tid = threadIdx.x;
+  u64 above = 0;  // count or mass of the keys over `high`
+  for (int step = 0; low < high; ++step) {
+    if (step == 8) {  // ranges that bins cannot tell apart: bit by bit
+      while (low < high) {
+        const unsigned t = low + (high - low) / 2;
+        u64 part = 0;
+        row.each([&](float v) {
+          if (order_key(v) > t) part += MASS ? weights.whole_of(v) : 1;
+        });
+        part = block_sum(part, lds.wave[0]);
+        if (MASS ? part <= limit : part < limit)
+          high = t;
+        else
+          low = t + 1;
+      }
+      u64 part = 0;
+      row.each([&](float v) {
+        if (order_key(v) > low) part += MASS ? weights.whole_of(v) : 1;
+      });
+      above = block_sum(part, lds.wave[0]);
+      break;
+    }
+    const float base = 0.5f * key_value(low);
+    const float scale =
+        fminf(kBins / (0.5f * key_value(high) - base), 3e38f);
+    auto bin_of = [&](float v) {
+      return min(kBins - 1, (int)((0.5f * v - base) * scale));
+    };
+    for (int i = tid; i < kBins; i += kThreads) {
+      lds.count[i] = 0;
+      if (MASS) lds.mass[i] = 0;
+    }
+    if (tid == 0) {
+      lds.listed = 0;
+      lds.low = ~0u;
+      lds.high = 0;
+    }
+    __syncthreads();
+    row.each([&](float v) {
+      const unsigned key = order_key(v);
+      if (key < low || key > high) return;
+      const int bin = bin_of(v);
+      if (MASS)
+        atomicAdd(&lds.mass[bin], weights.whole_of(v));
+      else
+        atomicAdd(&lds.count[bin], 1u);
+    });
+    __syncthreads();
+    // thread t has the bins from the top: 2t and 2t + 1
+    constexpr int kEach = kBins / kThreads;
+    u64 own[kEach], sum = 0;
+    for (int e = 0; e < kEach; ++e) {
+      const int bin = kBins - 1 - (tid * kEach + e);
+      own[e] = MASS ? lds.mass[bin] : lds.count[bin];
+      sum += own[e];
+    }
+    u64 upto = above + block_scan(sum, lds.wave[0]);
+    for (int e = 0; e < kEach; ++e) {
+      const bool here = MASS ? upto <= limit && upto + own[e] > limit
+                             : upto < limit && upto + own[e] >= limit;
+      if (here) {
+        lds.answer[0] = kBins - 1 - (tid * kEach + e);
+        lds.answer[1] = upto;
+      }
+      upto += own[e];
+    }
+    __syncthreads();
+    const int bin = (int)lds.answer[0];
+    above = lds.answer[1];
+    unsigned least = ~0u, most = 0;
+    row.each([&](float v) {
+      const unsigned key = order_key(v);
+      if (key < low || key > high || bin_of(v) != bin) return;
+      least = min(least, key);
+      most = max(most, key);
+      const unsigned at = atomicAdd(&lds.listed, 1u);
+      if (at < kList) {
+        lds.list_key[at] = key;
+        if (MASS) lds.list_weight[at] = weights.whole_of(v);
+      }
+    });
+    if (most) {
+      atomicMin(&lds.low, least);
+      atomicMax(&lds.high, most);
+    }
+    __syncthreads();
+    low = lds.low;
+    high = lds.high;
+    const int listed = (int)lds.listed;
+    if (low < high && listed <= kList) {
+      if (tid < listed) {
+        const unsigned key = lds.list_key[tid];
+        u64 over = above, equal = 0;
+        for (int j = 0; j < listed; ++j) {
+          const unsigned other = lds.list_key[j];
+          const u64 w = MASS ? lds.list_weight[j] : 1;
+          if (other > key) over += w;
+          if (other == key) equal += w;
+        }
+        if (MASS ? over <= limit && over + equal > limit
+                 : over < limit && over + equal >= limit) {
+          lds.answer[2] = key;
+          lds.answer[3] = over;
+        }
+      }
+      __syncthreads();
+      low = high = (unsigned)lds.answer[2];
+      above = lds.answer[3];
+    }
+    __syncthreads();
+  }
+  if (!MASS) return Cut{low, limit - above};
+  const u64 w = weights.whole_of(key_value(low));
+  return Cut{low, w ? (limit - above) / w + 1 : (u64)row.vocab};
+}
+
 template <typename T>
 __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
-  __shared__ u64 lds[kWaves];
-  const long row = blockIdx.x;
-  const T* x = (const T*)a.logits + row * a.row_stride;
+  __shared__ Lds lds;
+  const long number = blockIdx.x;
   const int tid = threadIdx.x, V = a.vocab;
+  const Row<T> row((const T*)a.logits + number * a.row_stride, V);
 
-  double temperature = a.temperature ? a.temperature[row] : a.temperature_s;
-  long top_k = a.top_k ? a.top_k[row] : a.top_k_s;
-  double top_p = a.top_p ? a.top_p[row] : a.top_p_s;
-  double min_p = a.min_p ? a.min_p[row] : a.min_p_s;
+  double temperature =
+      a.temperature ? a.temperature[number] : a.temperature_s;
+  long top_k = a.top_k ? a.top_k[number] : a.top_k_s;
+  const double top_p = a.top_p ? a.top_p[number] : a.top_p_s;
+  double min_p = a.min_p ? a.min_p[number] : a.min_p_s;
   if (!(temperature > 0.0)) {  // greedy
     temperature = 1.0;
     top_k = 1;
   }
   temperature = fmin(temperature, 1e30);
-  if (top_k <= 0 || top_k > V) top_k = V;
+  if (top_k <= 0) top_k = V;
   if (min_p > 1.0) min_p = 1.0;
 
-  unsigned key_max = 0;
-  u64 bad = 0;
-  for (int i = tid; i < V; i += kThreads) {
-    const float v = DTypeTraits<T>::to_float(x[i]);
-    bad += v != v;
-    key_max = max(key_max, order_key(v));
-  }
-  bad = block_sum(bad, lds);
-  for (int o = 32; o > 0; o >>= 1)
-    key_max = max(key_max, (unsigned)__shfl_xor((int)key_max, o, WAVE_SIZE));
-  __syncthreads();
-  if ((tid & 63) == 0) lds[tid >> 6] = key_max;
-  __syncthreads();
-  for (int w = 0; w < kWaves; ++w) key_max = max(key_max, (unsigned)lds[w]);
-  if (bad || key_max == order_key(-INFINITY)) {
-    if (tid == 0) a.out[row] = -1;
+  if (tid < 64) lds.power[tid] = exp2(tid / 64.0);
+  // extreme keys of the logits above -inf, and how many those are
+  unsigned high = 0, low = ~0u, some = 0, bad = 0;
+  row.each([&](float v) {
+    bad |= v != v;
+    const unsigned key = order_key(v);
+    high = max(high, key);
+    if (v > -INFINITY) {
+      low = min(low, key);
+      ++some;
+    }
+  });
+  auto larger = [](unsigned x, unsigned y) { return max(x, y); };
+  high = block_reduce(bad ? ~0u : high, lds.wave[0], larger);
+  if (high == ~0u || high == order_key(-INFINITY)) {
+    if (tid == 0) a.out[number] = -1;
     return;
   }
-  const float top = __uint_as_float(
-      key_max & 0x80000000u ? key_max & 0x7fffffffu : ~key_max);
-  const double inv = 1.0 / temperature;
-  const double unit = (double)(1ull << a.shift);
-  auto weight = [&](float v) {
-    return v == top ? 1.0 : exp(((double)v - (double)top) * inv);
-  };
-  auto whole = [&](double w) { return (u64)rint(w * unit); };
+  const float top = key_value(high);
+  const Weights weights{top, 64.0 * 1.4426950408889634 / temperature, a.shift,
+                        lds.power};
 
-  // tokens with a larger key than cut are kept, and the first `ties` of those
-  // with this key
-  unsigned cut = 0;
-  u64 ties = V;
-  if (top_k < V) {
-    for (int bit = 31; bit >= 0; --bit) {
-      const unsigned t = cut | (1u << bit);
-      u64 n = 0;
-      for (int i = tid; i < V; i += kThreads)
-        n += order_key(DTypeTraits<T>::to_float(x[i])) >= t;
-      if (block_sum(n, lds) >= (u64)top_k) cut = t;
-    }
-    u64 n = 0;
-    for (int i = tid; i < V; i += kThreads)
-      n += order_key(DTypeTraits<T>::to_float(x[i])) > cut;
-    ties = top_k - block_sum(n, lds);
+  const bool by_mass = top_p > 0.0 && top_p < 1.0;
+  Cut cut{0, (u64)V};
+  if (top == INFINITY) {  // the others weigh nothing
+    cut = Cut{high, (u64)top_k};
+  } else if (top_k == 1) {
+    cut = Cut{high, 1};
+  } else if (top_k < V || by_mass) {
+    low = block_reduce(low, lds.wave[1],
+                       [](unsigned x, unsigned y) { return min(x, y); });
+    const u64 above = block_sum((u64)some, lds.wave[0]);
+    cut.key = low;  // below come those that weigh nothing
+    if ((u64)top_k < above)
+      cut = find_cut<false>(lds, row, weights, low, high, (u64)top_k);
   }
-  if (top_p > 0.0 && top_p < 1.0) {
-    u64 mass = 0, at_cut = 0;
-    for (int i = tid; i < V; i += kThreads) {
-      const float v = DTypeTraits<T>::to_float(x[i]);
+  if (by_mass) {
+    u64 mass = 0, equal = 0;
+    unsigned next = ~0u;  // the least key over the cut
+    row.each([&](float v) {
       const unsigned key = order_key(v);
-      if (key > cut) mass += whole(weight(v));
-      at_cut += key == cut;
-    }
-    mass = block_sum(mass, lds);
-    at_cut = block_sum(at_cut, lds);
-    const float cut_value = __uint_as_float(
-        cut & 0x80000000u ? cut & 0x7fffffffu : ~cut);
-    if (at_cut) mass += min(ties, at_cut) * whole(weight(cut_value));
-    const u64 most = floor_u64(top_p * (double)mass, mass);
-    // the least key t whose larger tokens weigh at most `most`
-    unsigned low = cut, high = key_max;
-    while (low < high) {
-      const unsigned t = low + (high - low) / 2;
-      u64 m = 0;
-      for (int i = tid; i < V; i += kThreads) {
-        const float v = DTypeTraits<T>::to_float(x[i]);
-        if (order_key(v) > t) m += whole(weight(v));
+      if (key > cut.key) {
+        mass += weights.whole_of(v);
+        next = min(next, key);
       }
-      if (block_sum(m, lds) <= most) high = t; else low = t + 1;
+      equal += key == cut.key;
+    });
+    mass = block_sum(mass, lds.wave[0]);
+    equal = min(block_sum(equal, lds.wave[1]), cut.ties);
+    const u64 each = weights.whole_of(key_value(cut.key));
+    const u64 all = mass + equal * each;
+    const u64 most = floor_u64(top_p * (double)all, all);
+    if (mass <= most) {
+      if (each) cut.ties = min(cut.ties, (most - mass) / each + 1);
+    } else {
+      next = block_reduce(next, lds.wave[0], [](unsigned x, unsigned y) {
+        return min(x, y);
+      });
+      cut = find_cut<true>(lds, row, weights, next, high, most);
     }
-    u64 m = 0;
-    for (int i = tid; i < V; i += kThreads) {
-      const float v = DTypeTraits<T>::to_float(x[i]);
-      if (order_key(v) > low) m += whole(weight(v));
-    }
-    m = block_sum(m, lds);
-    const float value = __uint_as_float(
-        low & 0x80000000u ? low & 0x7fffffffu : ~low);
-    const u64 w = value == value ? whole(weight(value)) : 0;
-    const u64 kept = w ? (most - m) / w + 1 : (u64)V;
-    ties = low > cut ? kept : min(ties, kept);
-    cut = low;
   }
 
-  // each thread owns a run of indices, so that ties are counted in order
-  const int each = (V + kThreads - 1) / kThreads;
-  const int first = min(V, tid * each), last = min(V, first + each);
-  u64 equal = 0;
-  for (int i = first; i < last; ++i)
-    equal += order_key(DTypeTraits<T>::to_float(x[i])) == cut;
-  u64 rank = block_scan(equal, lds);
-  u64 sum = 0, rank0 = rank;
-  auto kept = [&](float v, u64& rank) -> u64 {
-    const unsigned key = order_key(v);
-    if (key < cut) return 0;
-    if (key == cut && rank++ >= ties) return 0;
-    const double w = weight(v);
-    return w < min_p ? 0 : whole(w);
+  auto weigh = [&](float v) -> u64 {
+    const double w = weights.of(v);
+    return w < min_p ? 0 : weights.whole(w);
   };
-  for (int i = first; i < last; ++i)
-    sum += kept(DTypeTraits<T>::to_float(x[i]), rank);
-  const u64 total = block_sum(sum, lds);
-  u64 upto = block_scan(sum, lds);
-  u64 target = floor_u64((double)a.uniform[row] * (double)total, total - 1);
+  const u64 tie_weight = weigh(key_value(cut.key));
+  // how the kept weights lie over the waves' runs
+  u64 sum = 0, equal = 0;
+  row.each([&](float v) {
+    const unsigned key = order_key(v);
+    if (key > cut.key) sum += weigh(v);
+    equal += key == cut.key;
+  });
+  for (int o = 32; o > 0; o >>= 1) {
+    sum += __shfl_xor(sum, o, WAVE_SIZE);
+    equal += __shfl_xor(equal, o, WAVE_SIZE);
+  }
+  __syncthreads();
+  if ((tid & 63) == 0) {
+    lds.wave[0][tid >> 6] = sum;
+    lds.wave[1][tid >> 6] = equal;
+  }
+  __syncthreads();
+  auto kept_ties = [&](u64 before, u64 n) {
+    return before >= cut.ties ? 0 : min(n, cut.ties - before);
+  };
+  u64 total = 0, ties = 0;
+  for (int w = 0; w < kWaves; ++w) {
+    total += lds.wave[0][w] + kept_ties(ties, lds.wave[1][w]) * tie_weight;
+    ties += lds.wave[1][w];
+  }
+  const u64 target =
+      floor_u64((double)a.uniform[number] * (double)total, total - 1);
+  u64 upto = 0;
+  ties = 0;
+  int owner = 0;
+  for (; owner < kWaves; ++owner) {
+    const u64 here = lds.wave[0][owner] +
+                     kept_ties(ties, lds.wave[1][owner]) * tie_weight;
+    if (target < upto + here) break;
+    upto += here;
+    ties += lds.wave[1][owner];
+  }
+  // all threads share that run, each a few neighbours
+  if (tid == owner * 64) {
+    lds.answer[0] = row.first;
+    lds.answer[1] = row.last;
+  }
+  __syncthreads();
+  const int run_low = (int)lds.answer[0], run_high = (int)lds.answer[1];
+  const int each = (run_high - run_low + kThreads - 1) / kThreads;
+  const int first = min(run_high, run_low + tid * each);
+  const int last = min(run_high, first + each);
+  sum = equal = 0;
+  for (int i = first; i < last; ++i) {
+    const float v = row.at(i);
+    const unsigned key = order_key(v);
+    if (key > cut.key) sum += weigh(v);
+    equal += key == cut.key;
+  }
+  u64 rank = ties + block_scan(equal, lds.wave[1]);
+  sum += kept_ties(rank, equal) * tie_weight;
+  upto += block_scan(sum, lds.wave[0]);
   if (upto <= target && target < upto + sum) {
     for (int i = first; i < last; ++i) {
-      upto += kept(DTypeTraits<T>::to_float(x[i]), rank0);
+      const float v = row.at(i);
+      const unsigned key = order_key(v);
+      if (key > cut.key)
+        upto += weigh(v);
+      else if (key == cut.key && rank++ < cut.ties)
+        upto += tie_weight;
       if (upto > target) {
-        a.out[row] = i;
+        a.out[number] = i;
         break;
       }
     }
