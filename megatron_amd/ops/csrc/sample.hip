@@ -8,9 +8,9 @@
 // whose kept weights up to and with it exceed u times all kept weights.
 //
 // Weights are whole numbers of 2^-shift (64 bits, shift = 62 - log2 of the
-// vocabulary): their sums are exact in any order, so that filters and draw
-// agree with each other and from run to run. Exponentials are taken in 64
-// bits, since a draw hangs on sums that lie next to a border.
+// vocabulary, 51 at most): their sums are exact in any order, so that filters
+// and draw agree with each other and from run to run. Exponentials are taken
+// in 64 bits, since a draw hangs on sums that lie next to a border.
 //
 // A row with a NaN, or with no logit above -inf, gives -1.
 
@@ -53,48 +53,78 @@ __device__ __forceinline__ float key_value(unsigned key) {
 }
 
 constexpr int kBins = 2048;
-constexpr int kList = 256;  // candidates that are ranked one against another
+constexpr int kList = 256;  // tokens that are ranked one against another
+
+__constant__ const double kPower[64] = {  // 2^(j / 64)
+    1.0, 1.0108892860517005, 1.0218971486541166, 1.0330248790212284,
+    1.0442737824274138, 1.0556451783605572, 1.0671404006768237, 1.0787607977571199,
+    1.0905077326652577, 1.102382583307841, 1.1143867425958924, 1.1265216186082418,
+    1.1387886347566916, 1.1511892299529827, 1.1637248587775775, 1.1763969916502812,
+    1.189207115002721, 1.202156731452703, 1.215247359980469, 1.22848053610687,
+    1.241857812073484, 1.255380757024691, 1.2690509571917332, 1.2828700160787783,
+    1.2968395546510096, 1.3109612115247644, 1.3252366431597413, 1.339667524053303,
+    1.3542555469368927, 1.3690024229745905, 1.383909881963832, 1.3989796725383112,
+    1.4142135623730951, 1.42961333839197, 1.4451808069770467, 1.460917794180647,
+    1.4768261459394993, 1.4929077282912648, 1.5091644275934228, 1.5255981507445384,
+    1.5422108254079407, 1.559004400237837, 1.5759808451078865, 1.593142151342267,
+    1.6104903319492543, 1.6280274218573478, 1.645755478153965, 1.6636765803267364,
+    1.681792830507429, 1.7001063537185235, 1.718619298122478, 1.7373338352737062,
+    1.7562521603732995, 1.7753764925265212, 1.7947090750031072, 1.8142521755003989,
+    1.8340080864093424, 1.8539791250833855, 1.8741676341103, 1.8945759815869656,
+    1.9152065613971474, 1.9360617934922943, 1.9571441241754002, 1.978456026387951};
+
+struct Token {
+  float v;
+  int index;
+  u64 weight;
+};
 
 struct Lds {
   u64 mass[kBins];
   unsigned count[kBins];
-  u64 list_weight[kList];
-  unsigned list_key[kList];
+  Token list[kList];
+  double power[64];
   u64 wave[2][kWaves];
-  double power[64];  // 2^(j / 64)
   u64 answer[4];
+  float extreme[2][kWaves];
+  unsigned some[kWaves];
   unsigned listed, low, high;
 };
 
-template <typename V, typename F>
-__device__ __forceinline__ V block_reduce(V v, u64* lds, F join) {
-  for (int o = 32; o > 0; o >>= 1) v = join(v, __shfl_xor(v, o, WAVE_SIZE));
+__device__ __forceinline__ u64 wave_sum(u64 v) {
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, WAVE_SIZE);
+  return v;
+}
+
+__device__ __forceinline__ u64 wave_scan(u64 v, int width) {
+  const int lane = threadIdx.x & 63;
+  for (int o = 1; o < width; o <<= 1) {
+    const u64 other = __shfl_up(v, o, WAVE_SIZE);
+    if (lane >= o) v += other;
+  }
+  return v;
+}
+
+__device__ __forceinline__ u64 block_sum(u64 v, u64* lds) {
+  v = wave_sum(v);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
   __syncthreads();
-  V all = (V)lds[0];
-  for (int w = 1; w < kWaves; ++w) all = join(all, (V)lds[w]);
+  u64 all = lds[threadIdx.x & (kWaves - 1)];
+  for (int o = kWaves / 2; o > 0; o >>= 1) all += __shfl_xor(all, o, WAVE_SIZE);
   return all;
-}
-
-template <typename V>
-__device__ __forceinline__ V block_sum(V v, u64* lds) {
-  return block_reduce(v, lds, [](V a, V b) { return a + b; });
 }
 
 // sum of the values of all threads before this one
 __device__ __forceinline__ u64 block_scan(u64 v, u64* lds) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  u64 up = v;
-  for (int o = 1; o < 64; o <<= 1) {
-    const u64 other = __shfl_up(up, o, WAVE_SIZE);
-    if (lane >= o) up += other;
-  }
+  const u64 up = wave_scan(v, 64);
   __syncthreads();
   if (lane == 63) lds[wave] = up;
   __syncthreads();
-  for (int w = 0; w < wave; ++w) up += lds[w];
-  return up - v;
+  const u64 waves = wave_scan(lane < wave ? lds[lane & (kWaves - 1)] : 0,
+                              kWaves);
+  return up - v + __shfl(waves, kWaves - 1, WAVE_SIZE);
 }
 
 __device__ __forceinline__ u64 floor_u64(double x, u64 most) {
@@ -117,7 +147,7 @@ struct Row {
     const int step = WAVE_SIZE * kVec;
     const int run = ((vocab + shift + kWaves - 1) / kWaves + step - 1) /
                     step * step;
-    const int wave = threadIdx.x >> 6;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     first = min(vocab, max(0, wave * run - shift));
     last = min(vocab, (wave + 1) * run - shift);
   }
@@ -126,114 +156,135 @@ struct Row {
     return DTypeTraits<T>::to_float(x[i]);
   }
 
+  // f(value, index) for every value of the wave's run
   template <typename F>
   __device__ __forceinline__ void each(F f) const {
     const int lane = threadIdx.x & 63;
+    union Vec {
+      uint4 u;
+      T t[kVec];
+    };
     // the run's begin lies on 16 bytes, but for the row's own
-    const int begin = first == 0 ? -shift : first;
-    for (int base = begin; base < last; base += kBatch * WAVE_SIZE * kVec) {
-      union {
-        uint4 u;
-        T t[kVec];
-      } v[kBatch];
+    int base = first == 0 ? -shift : first;
+    constexpr int kStep = WAVE_SIZE * kVec;
+    if (base < 0 && base + kStep <= last) {  // the row's begin
+      const int i = base + lane * kVec;
+      for (int e = 0; e < kVec; ++e)
+        if (i + e >= 0) f(at(i + e), i + e);
+      base += kStep;
+    }
+    if (base >= 0) {
+      for (; base + kBatch * kStep <= last; base += kBatch * kStep) {
+        Vec v[kBatch];
 #pragma unroll
-      for (int k = 0; k < kBatch; ++k) {
-        const int i = base + (k * WAVE_SIZE + lane) * kVec;
-        if (i >= 0 && i + kVec <= last) {
-          v[k].u = *(const uint4*)(x + i);
-        } else {
+        for (int k = 0; k < kBatch; ++k)
+          v[k].u = *(const uint4*)(x + base + (k * WAVE_SIZE + lane) * kVec);
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k)
 #pragma unroll
           for (int e = 0; e < kVec; ++e)
-            if (i + e >= 0 && i + e < last) v[k].t[e] = x[i + e];
-        }
+            f(DTypeTraits<T>::to_float(v[k].t[e]),
+              base + (k * WAVE_SIZE + lane) * kVec + e);
       }
-#pragma unroll
-      for (int k = 0; k < kBatch; ++k) {
-        const int i = base + (k * WAVE_SIZE + lane) * kVec;
+    }
+    for (; base < last; base += kStep) {
+      const int i = base + lane * kVec;
+      if (i >= 0 && i + kVec <= last) {
+        Vec v;
+        v.u = *(const uint4*)(x + i);
 #pragma unroll
         for (int e = 0; e < kVec; ++e)
-          if (i + e >= 0 && i + e < last)
-            f(DTypeTraits<T>::to_float(v[k].t[e]));
+          f(DTypeTraits<T>::to_float(v.t[e]), i + e);
+      } else {
+        for (int e = 0; e < kVec; ++e)
+          if (i + e >= 0 && i + e < last) f(at(i + e), i + e);
       }
     }
   }
 };
 
-// Weights of a row: 2^y with y = (x - top) / T log2 e <= 0, from a table of
-// 2^(j / 64) and a polynomial of the fourth degree on the rest, which is at
-// most ln 2 / 128 (relative error under 2^-44).
+// Weights of a row: 2^(y / 64) with y = 64 (x - top) / T log2 e <= 0, from a
+// table of 2^(j / 64) and a polynomial of the fourth degree on the rest,
+// which is at most ln 2 / 128 (relative error under 2^-44). As a whole number
+// of 2^-shift a weight is read off the low bits of its sum with 2^(52-shift).
 struct Weights {
   float top;
-  double per;  // log2 e / T, 64 times
-  int shift;
+  double per;   // 64 log2 e / T
+  double unit;  // 2^(52 - shift)
   const double* power;
 
   __device__ __forceinline__ double of(float v) const {
-    if (v == top) return 1.0;
-    const double y = fmax(((double)v - (double)top) * per, -64.0 * 1000.0);
-    const double k = rint(y);
-    const double r = (y - k) * (0.6931471805599453 / 64);
-    double p = fma(r, 1.0 / 24, 1.0 / 6);
-    p = fma(r, p, 0.5);
+    if (top == INFINITY) return v == top ? 1.0 : 0.0;
+    const double y = fmax(((double)v - (double)top) * per, -64000.0);
+    const double big = 6755399441055744.0;  // 1.5 * 2^52
+    const double k = y + big;
+    const double r = y - (k - big);
+    constexpr double c = 0.6931471805599453 / 64;
+    double p = fma(r, c * c * c * c / 24, c * c * c / 6);
+    p = fma(r, p, c * c / 2);
+    p = fma(r, p, c);
     p = fma(r, p, 1.0);
-    p = fma(r, p, 1.0);
-    const int n = (int)k;
-    return ldexp(p * power[n & 63], n >> 6);
+    const int n = (int)__double2loint(k);
+    const double q = power[n & 63];
+    return p * __hiloint2double(__double2hiint(q) + ((n & ~63) << 14),
+                                __double2loint(q));
   }
   __device__ __forceinline__ u64 whole(double w) const {
-    const double high = trunc(ldexp(w, shift - 32));
-    const unsigned h = (unsigned)high;
-    return (u64)h << 32 | (unsigned)ldexp(ldexp(w, shift - 32) - high, 32);
+    return (u64)(__double_as_longlong(w + unit) - __double_as_longlong(unit));
   }
   __device__ __forceinline__ u64 whole_of(float v) const {
     return whole(of(v));
   }
 };
 
-// Tokens with a larger key are kept, and the first `ties` of those with this.
+// Tokens with a larger logit are kept, and the first `ties` of those with
+// this one; or the list holds all that can be kept.
 struct Cut {
-  unsigned key;
+  float v;
   u64 ties;
+  int listed;
 };
 
-// Down from the largest key, where `limit` is passed: by count (MASS false)
-// the key of the limit-th token, by mass the least key whose larger ones weigh
-// at most `limit`. Tokens above `floor` count, which more than `limit` have;
-// low..high are their extreme keys, both finite.
+// Down from the largest logit, where `limit` is passed: by count (MASS false)
+// the limit-th token, by mass the least logit whose larger ones weigh at most
+// `limit`. low and high are the extremes of the tokens that count, finite;
+// more than `limit` of them there are.
 //
-// Each step shares the keys' range out over bins, finds the bin in which the
-// limit is passed and goes on within it, until it is one key or few tokens.
+// Each step shares the range out over bins, finds the bin in which the limit
+// is passed and goes on within it, until it holds one logit or few tokens; or,
+// with few tokens from there up, lists those.
 template <bool MASS, typename T>
 __device__ Cut find_cut(Lds& lds, const Row<T>& row, const Weights& weights,
-                        unsigned low, unsigned high, u64 limit) {
+                        float low, float high, u64 limit) {
   const int tid = threadIdx.x;
-  u64 above = 0;  // count or mass of the keys over `high`
+  u64 above = 0;     // count or mass of the tokens over `high`
+  unsigned over = 0;  // count of them
   for (int step = 0; low < high; ++step) {
-    if (step == 8) {  // ranges that bins cannot tell apart: bit by bit
-      while (low < high) {
-        const unsigned t = low + (high - low) / 2;
+    if (step == 8) {  // a range that bins cannot tell apart: bit by bit
+      unsigned l = order_key(low), h = order_key(high);
+      auto part_over = [&](unsigned t) {
         u64 part = 0;
-        row.each([&](float v) {
+        row.each([&](float v, int) {
           if (order_key(v) > t) part += MASS ? weights.whole_of(v) : 1;
         });
-        part = block_sum(part, lds.wave[0]);
+        return block_sum(part, lds.wave[0]);
+      };
+      while (l < h) {
+        const unsigned t = l + (h - l) / 2;
+        const u64 part = part_over(t);
         if (MASS ? part <= limit : part < limit)
-          high = t;
+          h = t;
         else
-          low = t + 1;
+          l = t + 1;
       }
-      u64 part = 0;
-      row.each([&](float v) {
-        if (order_key(v) > low) part += MASS ? weights.whole_of(v) : 1;
-      });
-      above = block_sum(part, lds.wave[0]);
+      above = part_over(l);
+      low = key_value(l);
       break;
     }
-    const float base = 0.5f * key_value(low);
-    const float scale =
-        fminf(kBins / (0.5f * key_value(high) - base), 3e38f);
-    auto bin_of = [&](float v) {
-      return min(kBins - 1, (int)((0.5f * v - base) * scale));
+    const float scale = fminf((kBins - 0.5f) / (high - low), 3e38f);
+    const float shift = -low * scale;
+    auto bin_of = [&](float v) {  // rises with v, rounding and all
+      return min(kBins - 1, max(0, (int)fmaf(v, scale, shift)));
     };
     for (int i = tid; i < kBins; i += kThreads) {
       lds.count[i] = 0;
@@ -245,47 +296,63 @@ __device__ Cut find_cut(Lds& lds, const Row<T>& row, const Weights& weights,
       lds.high = 0;
     }
     __syncthreads();
-    row.each([&](float v) {
-      const unsigned key = order_key(v);
-      if (key < low || key > high) return;
-      const int bin = bin_of(v);
-      if (MASS)
-        atomicAdd(&lds.mass[bin], weights.whole_of(v));
-      else
+    row.each([&](float v, int) {
+      if (v >= low && v <= high) {
+        const int bin = bin_of(v);
         atomicAdd(&lds.count[bin], 1u);
+        if (MASS) atomicAdd(&lds.mass[bin], weights.whole_of(v));
+      }
     });
     __syncthreads();
-    // thread t has the bins from the top: 2t and 2t + 1
+    // thread t has two bins, from the top
     constexpr int kEach = kBins / kThreads;
-    u64 own[kEach], sum = 0;
+    u64 own[kEach], sum = 0, tokens = 0;
     for (int e = 0; e < kEach; ++e) {
       const int bin = kBins - 1 - (tid * kEach + e);
       own[e] = MASS ? lds.mass[bin] : lds.count[bin];
       sum += own[e];
+      tokens += lds.count[bin];
     }
     u64 upto = above + block_scan(sum, lds.wave[0]);
+    u64 tokens_upto = over;
+    if (MASS) tokens_upto += block_scan(tokens, lds.wave[1]);
     for (int e = 0; e < kEach; ++e) {
+      const int bin = kBins - 1 - (tid * kEach + e);
+      if (!MASS) tokens_upto = upto;
       const bool here = MASS ? upto <= limit && upto + own[e] > limit
                              : upto < limit && upto + own[e] >= limit;
       if (here) {
-        lds.answer[0] = kBins - 1 - (tid * kEach + e);
+        lds.answer[0] = bin;
         lds.answer[1] = upto;
+        lds.answer[2] = tokens_upto;
+        lds.answer[3] = tokens_upto + lds.count[bin];
       }
       upto += own[e];
+      tokens_upto += lds.count[bin];
     }
     __syncthreads();
     const int bin = (int)lds.answer[0];
     above = lds.answer[1];
+    over = (unsigned)lds.answer[2];
+    if (lds.answer[3] <= kList) {  // all from this bin up
+      row.each([&](float v, int i) {
+        if (v > high || (v >= low && bin_of(v) >= bin)) {
+          const unsigned at = atomicAdd(&lds.listed, 1u);
+          lds.list[at] = Token{v, i, 0};
+        }
+      });
+      __syncthreads();
+      return Cut{0.f, 0, (int)lds.listed};
+    }
     unsigned least = ~0u, most = 0;
-    row.each([&](float v) {
-      const unsigned key = order_key(v);
-      if (key < low || key > high || bin_of(v) != bin) return;
-      least = min(least, key);
-      most = max(most, key);
-      const unsigned at = atomicAdd(&lds.listed, 1u);
-      if (at < kList) {
-        lds.list_key[at] = key;
-        if (MASS) lds.list_weight[at] = weights.whole_of(v);
+    row.each([&](float v, int i) {
+      if (v >= low && v <= high && bin_of(v) == bin) {
+        const unsigned key = order_key(v);
+        least = min(least, key);
+        most = max(most, key);
+        const unsigned at = atomicAdd(&lds.listed, 1u);
+        if (at < kList)
+          lds.list[at] = Token{v, i, MASS ? weights.whole_of(v) : 1};
       }
     });
     if (most) {
@@ -293,41 +360,99 @@ __device__ Cut find_cut(Lds& lds, const Row<T>& row, const Weights& weights,
       atomicMax(&lds.high, most);
     }
     __syncthreads();
-    low = lds.low;
-    high = lds.high;
+    low = key_value(lds.low);
+    high = key_value(lds.high);
     const int listed = (int)lds.listed;
     if (low < high && listed <= kList) {
-      if (tid < listed) {
-        const unsigned key = lds.list_key[tid];
-        u64 over = above, equal = 0;
-        for (int j = 0; j < listed; ++j) {
-          const unsigned other = lds.list_key[j];
-          const u64 w = MASS ? lds.list_weight[j] : 1;
-          if (other > key) over += w;
-          if (other == key) equal += w;
+      const int at = tid >> 2;  // four threads rank a token
+      if (at < listed) {
+        const float own_v = lds.list[at].v;
+        u64 larger = 0, equal = 0;
+        for (int j = tid & 3; j < listed; j += 4) {
+          const Token other = lds.list[j];
+          if (other.v > own_v) larger += other.weight;
+          if (other.v == own_v) equal += other.weight;
         }
-        if (MASS ? over <= limit && over + equal > limit
-                 : over < limit && over + equal >= limit) {
-          lds.answer[2] = key;
-          lds.answer[3] = over;
+        for (int o = 1; o < 4; o <<= 1) {
+          larger += __shfl_xor(larger, o, WAVE_SIZE);
+          equal += __shfl_xor(equal, o, WAVE_SIZE);
+        }
+        larger += above;
+        if (MASS ? larger <= limit && larger + equal > limit
+                 : larger < limit && larger + equal >= limit) {
+          lds.low = order_key(own_v);
+          lds.answer[3] = larger;
         }
       }
       __syncthreads();
-      low = high = (unsigned)lds.answer[2];
+      low = high = key_value(lds.low);
       above = lds.answer[3];
     }
     __syncthreads();
   }
-  if (!MASS) return Cut{low, limit - above};
-  const u64 w = weights.whole_of(key_value(low));
-  return Cut{low, w ? (limit - above) / w + 1 : (u64)row.vocab};
+  if (!MASS) return Cut{low, limit - above, -1};
+  const u64 w = weights.whole_of(low);
+  return Cut{low, w ? (limit - above) / w + 1 : (u64)row.vocab, -1};
+}
+
+// Draws from the listed tokens: ranks them, filters, and sums the kept ones in
+// the order of their indices. Four threads work for a token.
+__device__ void draw_listed(Lds& lds, const Weights& weights, int listed,
+                            u64 top_k, bool by_mass, bool known, u64 most,
+                            double top_p, double min_p, float uniform,
+                            long* out) {
+  const int tid = threadIdx.x, at = tid >> 2, part = tid & 3;
+  const bool mine = at < listed;
+  Token own{0.f, 0, 0};
+  double w = 0.0;
+  if (mine) {
+    own = lds.list[at];
+    w = weights.of(own.v);
+    own.weight = weights.whole(w);
+  }
+  __syncthreads();
+  if (mine && part == 0) lds.list[at].weight = own.weight;
+  __syncthreads();
+  auto over_parts = [&](auto f) {
+    u64 sum = 0;
+    if (mine)
+      for (int j = part; j < listed; j += 4) sum += f(lds.list[j]);
+    sum += __shfl_xor(sum, 1, WAVE_SIZE);
+    return sum + __shfl_xor(sum, 2, WAVE_SIZE);
+  };
+  auto before = [&](const Token& t) {
+    return t.v > own.v || (t.v == own.v && t.index < own.index);
+  };
+  const u64 rank = over_parts([&](const Token& t) { return (u64)before(t); });
+  bool keep = mine && rank < top_k;
+  if (by_mass) {
+    const u64 mass = over_parts(
+        [&](const Token& t) { return before(t) ? t.weight : 0; });
+    if (!known) {
+      const u64 all =
+          block_sum(keep && part == 0 ? own.weight : 0, lds.wave[0]);
+      most = floor_u64(top_p * (double)all, all);
+    }
+    keep &= mass <= most;
+  }
+  keep &= !(w < min_p);
+  __syncthreads();
+  if (mine && part == 0 && !keep) lds.list[at].weight = 0;
+  const u64 total =
+      block_sum(keep && part == 0 ? own.weight : 0, lds.wave[0]);
+  const u64 target = floor_u64((double)uniform * (double)total, total - 1);
+  const u64 upto = over_parts([&](const Token& t) {
+    return t.index < own.index ? t.weight : 0;
+  });
+  if (keep && part == 0 && upto <= target && target < upto + own.weight)
+    *out = own.index;
 }
 
 template <typename T>
 __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
   __shared__ Lds lds;
   const long number = blockIdx.x;
-  const int tid = threadIdx.x, V = a.vocab;
+  const int tid = threadIdx.x, V = a.vocab, lane = tid & 63, wave = tid >> 6;
   const Row<T> row((const T*)a.logits + number * a.row_stride, V);
 
   double temperature =
@@ -335,118 +460,168 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
   long top_k = a.top_k ? a.top_k[number] : a.top_k_s;
   const double top_p = a.top_p ? a.top_p[number] : a.top_p_s;
   double min_p = a.min_p ? a.min_p[number] : a.min_p_s;
+  const float uniform = a.uniform[number];
   if (!(temperature > 0.0)) {  // greedy
     temperature = 1.0;
     top_k = 1;
   }
   temperature = fmin(temperature, 1e30);
-  if (top_k <= 0) top_k = V;
+  if (top_k <= 0 || top_k > V) top_k = V;
   if (min_p > 1.0) min_p = 1.0;
+  const bool by_mass = top_p > 0.0 && top_p < 1.0 && top_k > 1;
+  const bool filtered = by_mass || (top_k > 1 && top_k < V);
 
-  if (tid < 64) lds.power[tid] = exp2(tid / 64.0);
-  // extreme keys of the logits above -inf, and how many those are
-  unsigned high = 0, low = ~0u, some = 0, bad = 0;
-  row.each([&](float v) {
-    bad |= v != v;
-    const unsigned key = order_key(v);
-    high = max(high, key);
-    if (v > -INFINITY) {
-      low = min(low, key);
-      ++some;
-    }
-  });
-  auto larger = [](unsigned x, unsigned y) { return max(x, y); };
-  high = block_reduce(bad ? ~0u : high, lds.wave[0], larger);
-  if (high == ~0u || high == order_key(-INFINITY)) {
+  if (tid < 64) lds.power[tid] = kPower[tid];
+  // extremes of the logits above -inf, and how many those are
+  float high = -INFINITY, low = INFINITY;
+  unsigned some = 0;
+  bool bad = false;
+  if (filtered) {
+    row.each([&](float v, int) {
+      bad |= v != v;
+      high = fmaxf(high, v);
+      if (v > -INFINITY) {
+        low = fminf(low, v);
+        ++some;
+      }
+    });
+  } else {
+    row.each([&](float v, int) {
+      bad |= v != v;
+      high = fmaxf(high, v);
+    });
+  }
+  if (bad) some = 1u << 31;
+  for (int o = 32; o > 0; o >>= 1) {
+    high = fmaxf(high, __shfl_xor(high, o, WAVE_SIZE));
+    low = fminf(low, __shfl_xor(low, o, WAVE_SIZE));
+    const unsigned other = __shfl_xor((int)some, o, WAVE_SIZE);
+    some = ((some + other) & 0x7fffffffu) | ((some | other) & 0x80000000u);
+  }
+  if (lane == 0) {
+    lds.extreme[0][wave] = high;
+    lds.extreme[1][wave] = low;
+    lds.some[wave] = some;
+  }
+  __syncthreads();
+  high = lds.extreme[0][lane & (kWaves - 1)];
+  low = lds.extreme[1][lane & (kWaves - 1)];
+  some = lds.some[lane & (kWaves - 1)];
+  for (int o = kWaves / 2; o > 0; o >>= 1) {
+    high = fmaxf(high, __shfl_xor(high, o, WAVE_SIZE));
+    low = fminf(low, __shfl_xor(low, o, WAVE_SIZE));
+    const unsigned other = __shfl_xor((int)some, o, WAVE_SIZE);
+    some = ((some + other) & 0x7fffffffu) | ((some | other) & 0x80000000u);
+  }
+  if (some >> 31 || high == -INFINITY) {
     if (tid == 0) a.out[number] = -1;
     return;
   }
-  const float top = key_value(high);
-  const Weights weights{top, 64.0 * 1.4426950408889634 / temperature, a.shift,
-                        lds.power};
+  const float top = high;
 
-  const bool by_mass = top_p > 0.0 && top_p < 1.0;
-  Cut cut{0, (u64)V};
+  if (top_k == 1) {  // the first of the largest
+    if (tid == 0) lds.low = ~0u;
+    __syncthreads();
+    unsigned at = ~0u;
+    row.each([&](float v, int i) {
+      if (v == top) at = min(at, (unsigned)i);
+    });
+    if (at != ~0u) atomicMin(&lds.low, at);
+    __syncthreads();
+    if (tid == 0) a.out[number] = lds.low;
+    return;
+  }
+
+  const Weights weights{
+      top, 64.0 * 1.4426950408889634 / temperature,
+      __longlong_as_double((long long)(1023 + 52 - a.shift) << 52),
+      lds.power};
+  Cut cut{-INFINITY, (u64)V, -1};
   if (top == INFINITY) {  // the others weigh nothing
-    cut = Cut{high, (u64)top_k};
-  } else if (top_k == 1) {
-    cut = Cut{high, 1};
-  } else if (top_k < V || by_mass) {
-    low = block_reduce(low, lds.wave[1],
-                       [](unsigned x, unsigned y) { return min(x, y); });
-    const u64 above = block_sum((u64)some, lds.wave[0]);
-    cut.key = low;  // below come those that weigh nothing
-    if ((u64)top_k < above)
+    cut = Cut{top, (u64)top_k, -1};
+  } else if (filtered) {
+    cut.v = low;  // below come those that weigh nothing
+    if (top_k < (long)some)
       cut = find_cut<false>(lds, row, weights, low, high, (u64)top_k);
   }
-  if (by_mass) {
+  bool known = false;
+  u64 most = 0;
+  if (by_mass && cut.listed < 0) {
     u64 mass = 0, equal = 0;
-    unsigned next = ~0u;  // the least key over the cut
-    row.each([&](float v) {
-      const unsigned key = order_key(v);
-      if (key > cut.key) {
+    float next = INFINITY;  // the least logit over the cut
+    row.each([&](float v, int) {
+      if (v > cut.v) {
         mass += weights.whole_of(v);
-        next = min(next, key);
+        next = fminf(next, v);
       }
-      equal += key == cut.key;
+      equal += v == cut.v;
     });
     mass = block_sum(mass, lds.wave[0]);
     equal = min(block_sum(equal, lds.wave[1]), cut.ties);
-    const u64 each = weights.whole_of(key_value(cut.key));
+    const u64 each = weights.whole_of(cut.v);
     const u64 all = mass + equal * each;
-    const u64 most = floor_u64(top_p * (double)all, all);
+    most = floor_u64(top_p * (double)all, all);
+    known = true;
     if (mass <= most) {
       if (each) cut.ties = min(cut.ties, (most - mass) / each + 1);
     } else {
-      next = block_reduce(next, lds.wave[0], [](unsigned x, unsigned y) {
-        return min(x, y);
-      });
+      for (int o = 32; o > 0; o >>= 1)
+        next = fminf(next, __shfl_xor(next, o, WAVE_SIZE));
+      if (lane == 0) lds.extreme[1][wave] = next;
+      __syncthreads();
+      for (int w = 0; w < kWaves; ++w) next = fminf(next, lds.extreme[1][w]);
       cut = find_cut<true>(lds, row, weights, next, high, most);
     }
+  }
+  if (cut.listed >= 0) {
+    draw_listed(lds, weights, cut.listed, (u64)top_k, by_mass, known, most,
+                top_p, min_p, uniform, a.out + number);
+    return;
   }
 
   auto weigh = [&](float v) -> u64 {
     const double w = weights.of(v);
     return w < min_p ? 0 : weights.whole(w);
   };
-  const u64 tie_weight = weigh(key_value(cut.key));
+  const u64 tie_weight = weigh(cut.v);
   // how the kept weights lie over the waves' runs
   u64 sum = 0, equal = 0;
-  row.each([&](float v) {
-    const unsigned key = order_key(v);
-    if (key > cut.key) sum += weigh(v);
-    equal += key == cut.key;
-  });
-  for (int o = 32; o > 0; o >>= 1) {
-    sum += __shfl_xor(sum, o, WAVE_SIZE);
-    equal += __shfl_xor(equal, o, WAVE_SIZE);
+  if (cut.v == -INFINITY && !(min_p > 0.0)) {
+    row.each([&](float v, int) { sum += weights.whole_of(v); });
+  } else {
+    row.each([&](float v, int) {
+      if (v > cut.v) sum += weigh(v);
+      equal += v == cut.v;
+    });
   }
+  sum = wave_sum(sum);
+  equal = wave_sum(equal);
   __syncthreads();
-  if ((tid & 63) == 0) {
-    lds.wave[0][tid >> 6] = sum;
-    lds.wave[1][tid >> 6] = equal;
+  if (lane == 0) {
+    lds.wave[0][wave] = sum;
+    lds.wave[1][wave] = equal;
   }
   __syncthreads();
   auto kept_ties = [&](u64 before, u64 n) {
     return before >= cut.ties ? 0 : min(n, cut.ties - before);
   };
-  u64 total = 0, ties = 0;
-  for (int w = 0; w < kWaves; ++w) {
-    total += lds.wave[0][w] + kept_ties(ties, lds.wave[1][w]) * tie_weight;
-    ties += lds.wave[1][w];
-  }
+  // every wave finds the run with the target, a lane for each run
+  const int run = lane & (kWaves - 1);
+  const u64 run_ties = lds.wave[1][run];
+  const u64 ties_before = wave_scan(lane < kWaves ? run_ties : 0, kWaves) -
+                          (lane < kWaves ? run_ties : 0);
+  const u64 own =
+      lane < kWaves
+          ? lds.wave[0][run] + kept_ties(ties_before, run_ties) * tie_weight
+          : 0;
+  const u64 run_upto = wave_scan(own, kWaves);
+  const u64 total = __shfl(run_upto, kWaves - 1, WAVE_SIZE);
   const u64 target =
-      floor_u64((double)a.uniform[number] * (double)total, total - 1);
-  u64 upto = 0;
-  ties = 0;
-  int owner = 0;
-  for (; owner < kWaves; ++owner) {
-    const u64 here = lds.wave[0][owner] +
-                     kept_ties(ties, lds.wave[1][owner]) * tie_weight;
-    if (target < upto + here) break;
-    upto += here;
-    ties += lds.wave[1][owner];
-  }
+      floor_u64((double)uniform * (double)total, total - 1);
+  const int owner =
+      __builtin_ctzl(__ballot(lane < kWaves && target < run_upto));
+  u64 upto = __shfl(run_upto - own, owner, WAVE_SIZE);
+  const u64 ties = __shfl(ties_before, owner, WAVE_SIZE);
   // all threads share that run, each a few neighbours
   if (tid == owner * 64) {
     lds.answer[0] = row.first;
@@ -460,9 +635,8 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
   sum = equal = 0;
   for (int i = first; i < last; ++i) {
     const float v = row.at(i);
-    const unsigned key = order_key(v);
-    if (key > cut.key) sum += weigh(v);
-    equal += key == cut.key;
+    if (v > cut.v) sum += weigh(v);
+    equal += v == cut.v;
   }
   u64 rank = ties + block_scan(equal, lds.wave[1]);
   sum += kept_ties(rank, equal) * tie_weight;
@@ -470,10 +644,9 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
   if (upto <= target && target < upto + sum) {
     for (int i = first; i < last; ++i) {
       const float v = row.at(i);
-      const unsigned key = order_key(v);
-      if (key > cut.key)
+      if (v > cut.v)
         upto += weigh(v);
-      else if (key == cut.key && rank++ < cut.ties)
+      else if (v == cut.v && rank++ < cut.ties)
         upto += tie_weight;
       if (upto > target) {
         a.out[number] = i;
@@ -516,7 +689,7 @@ torch::Tensor sample_tokens(torch::Tensor logits, torch::Tensor uniform,
   a.uniform = uniform.data_ptr<float>();
   a.out = out.data_ptr<long>();
   a.vocab = (int)v;
-  a.shift = 62;
+  a.shift = 51;
   while (v > (1l << (62 - a.shift))) --a.shift;
   auto f = [](const c10::optional<torch::Tensor>& t) {
     return t.has_value() ? t->data_ptr<float>() : nullptr;

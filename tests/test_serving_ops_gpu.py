@@ -580,6 +580,66 @@ def test_sample_infinities_and_nan():
     assert int(got[2]) < 100 and int(got[3]) in (5, 9) and int(got[4]) == 399
 
 
+@pytest.mark.parametrize("kind", ["floor", "masked", "offset", "tiny", "two",
+                                  "steps", "wide"])
+def test_sample_ranges_that_are_hard_to_share_out(kind):
+    """Logits of which most are far from the others, or next to each other."""
+    g = generator(25)
+    b, vocab = 5, 3001
+    logits = randn(g, b, vocab)
+    if kind == "floor":  # masked by the type's lowest value
+        logits[:, 500:] = torch.finfo(FP32).min
+    elif kind == "masked":
+        logits[torch.rand(b, vocab, generator=g) < 0.5] = -1e4
+    elif kind == "offset":
+        logits = 1000 + logits * 1e-3
+    elif kind == "tiny":  # all within the subnormal numbers
+        logits = logits * 1e-40
+    elif kind == "two":
+        logits = (logits > 0).float() * 1e-30
+    elif kind == "steps":
+        logits = (logits * 4).round() / 4
+    else:
+        logits = logits * 1e38
+    u = torch.rand(b, generator=g)
+    for top_k, top_p, min_p in FILTERS + [(400, 0.0, 0.0), (2000, 0.7, 0.0)]:
+        got = sample_tokens(logits.cuda(), u.cuda(), top_k=top_k,
+                            top_p=top_p, min_p=min_p)
+        want = [sample_exact(logits[i], float(u[i]), 1.0, top_k, top_p,
+                             min_p) for i in range(b)]
+        assert got.tolist() == want, (top_k, top_p, min_p)
+
+
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+@pytest.mark.parametrize("offset", [1, 2, 3, 5, 7])
+def test_sample_rows_that_begin_anywhere(dtype, offset):
+    g = generator(26)
+    b, vocab = 4, 4999
+    wide = (randn(g, b, vocab + 11) * 2).to(dtype)
+    u = torch.rand(b, generator=g)
+    rows = wide.cuda()[:, offset:offset + vocab]
+    for top_k, top_p, min_p in ((0, 0.0, 0.0), (33, 0.0, 0.0),
+                                (0, 0.9, 0.0), (600, 0.9, 0.02),
+                                (1, 0.0, 0.0)):
+        got = sample_tokens(rows, u.cuda(), 0.8, top_k, top_p, min_p)
+        want = [sample_exact(wide[i, offset:offset + vocab], float(u[i]),
+                             0.8, top_k, top_p, min_p) for i in range(b)]
+        assert got.tolist() == want
+
+
+def test_sample_largest_vocabulary():
+    g = generator(27)
+    vocab = 1 << 20
+    logits = randn(g, 2, vocab) * 2
+    u = torch.rand(2, generator=g)
+    for top_k, top_p in ((0, 0.0), (0, 0.95), (5000, 0.9), (20, 0.0)):
+        got = sample_tokens(logits.cuda(), u.cuda(), top_k=top_k,
+                            top_p=top_p)
+        want = [sample_exact(logits[i], float(u[i]), 1.0, top_k, top_p, 0.0)
+                for i in range(2)]
+        assert got.tolist() == want
+
+
 def test_sample_uniform_outside_still_falls_on_a_kept_token():
     logits = torch.zeros(4, 100)
     logits[:, 20:30] = 5.0
