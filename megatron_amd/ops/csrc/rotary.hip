@@ -26,7 +26,8 @@ struct RotaryTensor {
   int heads;
 };
 
-// One thread per pair or, past the pairs, per copied value.
+// One thread per pair or, past the pairs, per copied value: any strides and
+// widths.
 template <typename T>
 __global__ __launch_bounds__(256) void rotary_kernel(
     RotaryTensor q, RotaryTensor k, const float* __restrict__ cos_t,
@@ -62,6 +63,91 @@ __global__ __launch_bounds__(256) void rotary_kernel(
     const float x2 = DTypeTraits<T>::to_float(x[i2]);
     y[i1] = DTypeTraits<T>::from_float(x1 * c - x2 * s);
     y[i2] = DTypeTraits<T>::from_float(x2 * c + x1 * s);
+  }
+}
+
+// 16 bytes a lane. A workgroup takes one token and a run of heads: each thread
+// keeps its place in the head, so that the tables' values stay in registers
+// while it goes from head to head, four of them in flight.
+//
+// A unit is a vector of a head (interleaved: its pairs are in it; past the
+// pairs: copied) or, in the half layout, a vector and its partners r further.
+template <typename T, bool INTERLEAVED>
+__global__ __launch_bounds__(256) void rotary_vec_kernel(
+    RotaryTensor q, RotaryTensor k, const float* __restrict__ cos_t,
+    const float* __restrict__ sin_t, const long* __restrict__ positions,
+    long p_bs, long p_ss, int b, int h, int r, long table_rows, float sign,
+    int heads_each) {
+  constexpr int kVec = 16 / sizeof(T);
+  constexpr int kTurns = INTERLEAVED ? kVec / 2 : kVec;  // table values
+  constexpr int kFlight = 4;
+  using Vec = union {
+    uint4 u;
+    T t[kVec];
+  };
+  const int units = (INTERLEAVED ? h : h - r) / kVec;
+  const int side = 256 / units;  // heads side by side
+  const int unit = threadIdx.x % units;
+  const int line = threadIdx.x / units;
+  if (line >= side) return;
+  const long token = blockIdx.x;
+  const int is = (unsigned)token / (unsigned)b;
+  const int ib = token - (long)is * b;
+  const int heads = q.heads + k.heads;
+  const int first = blockIdx.y * heads_each + line;
+  const int last = min(heads, (int)(blockIdx.y + 1) * heads_each);
+  // where the unit lies, and whether it turns
+  const bool turns = INTERLEAVED ? unit * kVec < 2 * r : unit * kVec < r;
+  const int at = INTERLEAVED || turns ? unit * kVec : unit * kVec + r;
+
+  float c[kTurns], s[kTurns];
+  if (turns) {
+    const long p = positions ? positions[ib * p_bs + is * p_ss] : is;
+    const bool inside = p >= 0 && p < table_rows;
+    const int j = INTERLEAVED ? at / 2 : at;
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i) {
+      c[i] = inside ? cos_t[p * r + j + i] : NAN;
+      s[i] = inside ? sin_t[p * r + j + i] * sign : NAN;
+    }
+  }
+  for (int base = first; base < last; base += kFlight * side) {
+    Vec x[kFlight], z[kFlight];
+#pragma unroll
+    for (int f = 0; f < kFlight; ++f) {
+      const int head = base + f * side;
+      if (head < last) {
+        const bool is_q = head < q.heads;
+        const T* from =
+            is_q ? (const T*)q.x + is * q.ss + ib * q.bs + head * q.ns
+                 : (const T*)k.x + is * k.ss + ib * k.bs +
+                       (head - q.heads) * k.ns;
+        x[f].u = *(const uint4*)(from + at);
+        if (!INTERLEAVED && turns) z[f].u = *(const uint4*)(from + at + r);
+      }
+    }
+#pragma unroll
+    for (int f = 0; f < kFlight; ++f) {
+      const int head = base + f * side;
+      if (head < last) {
+        const bool is_q = head < q.heads;
+        T* to = is_q ? (T*)q.y + (token * q.heads + head) * h
+                     : (T*)k.y + (token * k.heads + head - q.heads) * h;
+        if (turns) {
+#pragma unroll
+          for (int i = 0; i < kTurns; ++i) {
+            T& t1 = INTERLEAVED ? x[f].t[2 * i] : x[f].t[i];
+            T& t2 = INTERLEAVED ? x[f].t[2 * i + 1] : z[f].t[i];
+            const float x1 = DTypeTraits<T>::to_float(t1);
+            const float x2 = DTypeTraits<T>::to_float(t2);
+            t1 = DTypeTraits<T>::from_float(x1 * c[i] - x2 * s[i]);
+            t2 = DTypeTraits<T>::from_float(x2 * c[i] + x1 * s[i]);
+          }
+          if (!INTERLEAVED) *(uint4*)(to + at + r) = z[f].u;
+        }
+        *(uint4*)(to + at) = x[f].u;
+      }
+    }
   }
 }
 
@@ -117,6 +203,47 @@ std::vector<torch::Tensor> rotary_apply(
   const long total = s * b * (tq.heads + tk.heads) * (long)(h - r);
   if (total == 0) return out;
   auto stream = c10::hip::getCurrentHIPStream();
+
+  // vectors: all rows on 16 bytes, and pairs that fill whole vectors
+  const int vec = 16 / (int)q.element_size();
+  auto wide = [&](const RotaryTensor& t) {
+    return (unsigned long)t.x % 16 == 0 && t.ss % vec == 0 &&
+           t.bs % vec == 0 && t.ns % vec == 0;
+  };
+  const int units = (interleaved ? h : h - r) / vec;
+  if (wide(tq) && wide(tk) && h % vec == 0 &&
+      (interleaved ? 2 * r : r) % vec == 0 && units <= 256 &&
+      s * b < (1l << 31)) {
+    // a workgroup goes over all heads of a token, unless there are so few
+    // tokens that their heads have to fill the card (at 16 tokens of 40 heads
+    // one round each takes 3.0 us, all rounds 3.3)
+    const int heads = tq.heads + tk.heads, side = 256 / units;
+    const int rounds = (heads + side - 1) / side;
+    const int split =
+        (int)std::max<long>(1, std::min<long>(rounds, 2048 / (s * b)));
+    const int heads_each = (rounds + split - 1) / split * side;
+    const dim3 grid((unsigned)(s * b), (heads + heads_each - 1) / heads_each);
+#define LAUNCH_ROTARY_VEC(T, I)                                              \
+  hipLaunchKernelGGL((rotary_vec_kernel<T, I>), grid, dim3(256), 0, stream,  \
+                     tq, tk, cos.data_ptr<float>(), sin.data_ptr<float>(),   \
+                     pos, p_bs, p_ss, (int)b, h, r, rows,                    \
+                     inverse ? -1.f : 1.f, heads_each)
+#define LAUNCH_ROTARY_LAYOUT(T)                                              \
+  do {                                                                       \
+    if (interleaved) LAUNCH_ROTARY_VEC(T, true);                             \
+    else LAUNCH_ROTARY_VEC(T, false);                                        \
+  } while (0)
+    switch (q.scalar_type()) {
+      case torch::kFloat32: LAUNCH_ROTARY_LAYOUT(float); break;
+      case torch::kBFloat16: LAUNCH_ROTARY_LAYOUT(__hip_bfloat16); break;
+      case torch::kFloat16: LAUNCH_ROTARY_LAYOUT(__half); break;
+      default: TORCH_CHECK(false, "rotary: fp32, bf16 or fp16 only");
+    }
+#undef LAUNCH_ROTARY_LAYOUT
+#undef LAUNCH_ROTARY_VEC
+    HIP_CHECK(hipGetLastError());
+    return out;
+  }
   const int grid = (int)std::min<long>((total + 255) / 256, 32768);
 #define LAUNCH_ROTARY(T)                                                     \
   hipLaunchKernelGGL((rotary_kernel<T>), dim3(grid), dim3(256), 0, stream,   \
