@@ -387,40 +387,51 @@ def rotate_reference(x, cos, sin, interleaved):
     return torch.cat([y.to(x.dtype), rest], dim=-1)
 
 
+def _rotate_pair(query, key, cos, sin, positions, interleaved, inverse):
+    """query and key (either may be None) turned, or turned back."""
+    ext = _C(cos)
+    if ext is not None:
+        # the kernel reads strided views with a dense head_dim
+        given = [t if t.stride(-1) == 1 else t.contiguous()
+                 for t in (query, key) if t is not None]
+        out = ext.rotary_apply(given[0], given[1] if len(given) > 1 else None,
+                               cos, sin, positions, interleaved, inverse)
+        if query is None:
+            return None, out[0]
+        return out[0], (out[1] if key is not None else None)
+    if positions is None:
+        s = (query if query is not None else key).shape[0]
+        c, s = (t[:s].unsqueeze(1) for t in (cos, sin))
+    else:
+        c, s = (t[positions.t()] for t in (cos, sin))
+    if inverse:
+        s = -s
+    return tuple(None if t is None else rotate_reference(t, c, s, interleaved)
+                 for t in (query, key))
+
+
+_ROTARY_TYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+
 class RotaryFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, query, key, cos, sin, positions, interleaved, inverse):
         ctx.save_for_backward(cos, sin, positions)
         ctx.mode = (interleaved, inverse)
         ctx.set_materialize_grads(False)
-        ext = _C(query)
-        if ext is not None:
-            # the kernel reads strided views with a dense head_dim
-            q, k = (t if t is None or t.stride(-1) == 1 else t.contiguous()
-                    for t in (query, key))
-            out = ext.rotary_apply(q, k, cos, sin, positions, interleaved,
-                                   inverse)
-            return out[0], (out[1] if key is not None else None)
-        if positions is None:
-            c, s = (t[: query.shape[0]].unsqueeze(1) for t in (cos, sin))
-        else:
-            c, s = (t[positions.t()] for t in (cos, sin))
-        if inverse:
-            s = -s
-        return (rotate_reference(query, c, s, interleaved),
-                rotate_reference(key, c, s, interleaved)
-                if key is not None else None)
+        return _rotate_pair(query, key, cos, sin, positions, interleaved,
+                            inverse)
 
     @staticmethod
     def backward(ctx, dq, dk):
         # the transpose of the rotation: the same with the angle negated
-        cos, sin, positions = ctx.saved_tensors
-        interleaved, inverse = ctx.mode
-        rest = (cos, sin, positions, interleaved, not inverse)
-        if dq is None and dk is not None:
-            dk, _ = RotaryFunction.apply(dk, None, *rest)
-        elif dq is not None:
-            dq, dk = RotaryFunction.apply(dq, dk, *rest)
+        if dq is not None or dk is not None:
+            cos, sin, positions = ctx.saved_tensors
+            interleaved, inverse = ctx.mode
+            turn = (RotaryFunction.apply if torch.is_grad_enabled()
+                    else _rotate_pair)
+            dq, dk = turn(dq, dk, cos, sin, positions, interleaved,
+                          not inverse)
         return dq, dk, None, None, None, None, None
 
 
@@ -437,34 +448,33 @@ def rotary_embedding(query, key, cos, sin, positions=None, interleaved=True):
     if query.dim() != 4:
         raise ValueError("query must be [s, b, heads, head_dim]")
     s, b, _, h = query.shape
-    if query.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+    dtype, device = query.dtype, query.device
+    if dtype not in _ROTARY_TYPES:
         raise ValueError(f"rotary_embedding takes fp32, bf16 or fp16, not "
-                         f"{query.dtype}")
+                         f"{dtype}")
     if key is not None and (
-            key.dim() != 4 or key.shape[:2] != query.shape[:2]
-            or key.shape[3] != h or key.dtype != query.dtype
-            or key.device != query.device):
+            key.dim() != 4 or key.shape[0] != s or key.shape[1] != b
+            or key.shape[3] != h or key.dtype != dtype
+            or key.device != device):
         raise ValueError("key must match the query but for its heads")
-    for t in (cos, sin):
-        if (t.dim() != 2 or t.dtype != torch.float32 or t.shape != cos.shape
-                or t.device != query.device
-                or not 1 <= t.shape[1] <= h // 2):
-            raise ValueError("cos and sin must be float32 [positions, up to "
-                             f"{h // 2}] on {query.device}")
-        if t.requires_grad:
-            raise ValueError("cos and sin have no gradient")
+    rows, r = cos.shape if cos.dim() == 2 else (0, 0)
+    if (not 1 <= r <= h // 2 or sin.shape != cos.shape
+            or cos.dtype != torch.float32 or sin.dtype != torch.float32
+            or cos.device != device or sin.device != device):
+        raise ValueError("cos and sin must be float32 [positions, up to "
+                         f"{h // 2}] on {device}")
+    if cos.requires_grad or sin.requires_grad:
+        raise ValueError("cos and sin have no gradient")
     if positions is None:
-        if cos.shape[0] < s:
-            raise ValueError(f"tables of {cos.shape[0]} positions for {s} "
-                             "tokens")
+        if rows < s:
+            raise ValueError(f"tables of {rows} positions for {s} tokens")
     else:
         if (positions.shape != (b, s) or positions.dtype != torch.int64
-                or positions.device != query.device):
+                or positions.device != device):
             raise ValueError(f"positions must be int64 [{b}, {s}] on "
-                             f"{query.device}")
+                             f"{device}")
         if not positions.is_cuda and positions.numel() and (
-                int(positions.min()) < 0
-                or int(positions.max()) >= cos.shape[0]):
+                int(positions.min()) < 0 or int(positions.max()) >= rows):
             raise ValueError("a position lies outside the tables")
     return RotaryFunction.apply(query, key, cos.contiguous(),
                                 sin.contiguous(), positions, interleaved,
