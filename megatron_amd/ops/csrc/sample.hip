@@ -72,6 +72,9 @@ __constant__ const double kPower[64] = {  // 2^(j / 64)
     1.7562521603732995, 1.7753764925265212, 1.7947090750031072, 1.8142521755003989,
     1.8340080864093424, 1.8539791250833855, 1.8741676341103, 1.8945759815869656,
     1.9152065613971474, 1.9360617934922943, 1.9571441241754002, 1.978456026387951};
+__constant__ const double kFine[4] = {  // 2^(j / 256)
+    1.0, 1.0027112750502025,
+    1.0054299011128027, 1.0081558981184175};
 
 struct Token {
   float v;
@@ -83,26 +86,72 @@ struct Lds {
   u64 mass[kBins];
   unsigned count[kBins];
   Token list[kList];
-  double power[64];
+  double power[256];
   u64 wave[2][kWaves];
   u64 answer[4];
   float extreme[2][kWaves];
-  unsigned some[kWaves];
   unsigned listed, low, high;
 };
 
-__device__ __forceinline__ u64 wave_sum(u64 v) {
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, WAVE_SIZE);
+// Joins a wave's values by row shifts and broadcasts: lane i gets those of the
+// lanes up to i, `none` standing for lanes that are not there. With ROW within
+// 16 lanes only.
+template <bool ROW = false, typename F>
+__device__ __forceinline__ unsigned wave_join(unsigned v, unsigned none,
+                                              F join) {
+#define JOIN_STEP(CTRL, ROWS)                                                \
+  v = join(v, (unsigned)__builtin_amdgcn_update_dpp((int)none, (int)v, CTRL, \
+                                                    ROWS, 0xf, false))
+  JOIN_STEP(0x111, 0xf);  // from 1, 2, 4, 8 lanes below, within 16
+  JOIN_STEP(0x112, 0xf);
+  JOIN_STEP(0x114, 0xf);
+  JOIN_STEP(0x118, 0xf);
+  if (!ROW) {
+    JOIN_STEP(0x142, 0xa);  // from the last lane of the 16 below
+    JOIN_STEP(0x143, 0xc);  // from lane 31
+  }
+#undef JOIN_STEP
   return v;
 }
 
-__device__ __forceinline__ u64 wave_scan(u64 v, int width) {
-  const int lane = threadIdx.x & 63;
-  for (int o = 1; o < width; o <<= 1) {
-    const u64 other = __shfl_up(v, o, WAVE_SIZE);
-    if (lane >= o) v += other;
+template <bool ROW = false>
+__device__ __forceinline__ u64 wave_scan(u64 v) {
+#define SCAN_STEP(CTRL, ROWS)                                               \
+  v += (u64)(unsigned)__builtin_amdgcn_update_dpp(0, (int)(v >> 32), CTRL,  \
+                                                  ROWS, 0xf, false)         \
+           << 32 |                                                          \
+       (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf,    \
+                                             false)
+  SCAN_STEP(0x111, 0xf);
+  SCAN_STEP(0x112, 0xf);
+  SCAN_STEP(0x114, 0xf);
+  SCAN_STEP(0x118, 0xf);
+  if (!ROW) {
+    SCAN_STEP(0x142, 0xa);
+    SCAN_STEP(0x143, 0xc);
   }
+#undef SCAN_STEP
   return v;
+}
+
+__device__ __forceinline__ u64 lane_value(u64 v, int lane) {
+  return (u64)(unsigned)__builtin_amdgcn_readlane((int)(v >> 32), lane)
+             << 32 |
+         (unsigned)__builtin_amdgcn_readlane((int)v, lane);
+}
+
+__device__ __forceinline__ u64 wave_sum(u64 v) {
+  return lane_value(wave_scan(v), 63);
+}
+
+__device__ __forceinline__ float wave_max(float v) {
+  return __uint_as_float(__builtin_amdgcn_readlane(
+      (int)wave_join(__float_as_uint(v), __float_as_uint(-INFINITY),
+                     [](unsigned x, unsigned y) {
+                       return __float_as_uint(
+                           fmaxf(__uint_as_float(x), __uint_as_float(y)));
+                     }),
+      63));
 }
 
 __device__ __forceinline__ u64 block_sum(u64 v, u64* lds) {
@@ -110,21 +159,20 @@ __device__ __forceinline__ u64 block_sum(u64 v, u64* lds) {
   __syncthreads();
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
   __syncthreads();
-  u64 all = lds[threadIdx.x & (kWaves - 1)];
-  for (int o = kWaves / 2; o > 0; o >>= 1) all += __shfl_xor(all, o, WAVE_SIZE);
-  return all;
+  return lane_value(wave_scan<true>(lds[threadIdx.x & (kWaves - 1)]),
+                    kWaves - 1);
 }
 
 // sum of the values of all threads before this one
 __device__ __forceinline__ u64 block_scan(u64 v, u64* lds) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const u64 up = wave_scan(v, 64);
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const u64 up = wave_scan(v);
   __syncthreads();
   if (lane == 63) lds[wave] = up;
   __syncthreads();
-  const u64 waves = wave_scan(lane < wave ? lds[lane & (kWaves - 1)] : 0,
-                              kWaves);
-  return up - v + __shfl(waves, kWaves - 1, WAVE_SIZE);
+  const u64 waves = wave_scan<true>(lds[lane & (kWaves - 1)]);
+  return up - v + (wave ? lane_value(waves, wave - 1) : 0);
 }
 
 __device__ __forceinline__ u64 floor_u64(double x, u64 most) {
@@ -203,37 +251,46 @@ struct Row {
   }
 };
 
-// Weights of a row: 2^(y / 64) with y = 64 (x - top) / T log2 e <= 0, from a
-// table of 2^(j / 64) and a polynomial of the fourth degree on the rest,
-// which is at most ln 2 / 128 (relative error under 2^-44). As a whole number
-// of 2^-shift a weight is read off the low bits of its sum with 2^(52-shift).
+// Weights of a row: 2^(y / 256) with y = 256 (x - top) / T log2 e <= 0, from a
+// table of 2^(j / 256) and a polynomial of the third degree on the rest, which
+// is at most ln 2 / 512 (relative error under 2^-42). As a whole number of
+// 2^-shift a weight is read off the low bits of its sum with 2^(52-shift).
+using LdsDouble = const __attribute__((address_space(3))) double;
+
 struct Weights {
-  float top;
-  double per;   // 64 log2 e / T
-  double unit;  // 2^(52 - shift)
-  const double* power;
+  double top, per;  // 256 log2 e / T
+  double unit;      // 2^(52 - shift)
+  double big, c1, c2, c3;
+  LdsDouble* power;
+
+  __device__ Weights(float top_, double temperature, int shift, Lds& lds)
+      : top(top_),
+        per(256.0 * 1.4426950408889634 / temperature),
+        unit(__longlong_as_double((long long)(1023 + 52 - shift) << 52)),
+        power((LdsDouble*)lds.power) {
+    constexpr double c = 0.6931471805599453 / 256;
+    big = 6755399441055744.0;  // 1.5 * 2^52
+    c1 = c, c2 = c * c / 2, c3 = c * c * c / 6;
+    // held in registers: fewer moves than from constants
+    asm("" : "+v"(big), "+v"(c1), "+v"(c2), "+v"(c3));
+  }
 
   __device__ __forceinline__ double of(float v) const {
-    if (top == INFINITY) return v == top ? 1.0 : 0.0;
-    const double y = fmax(((double)v - (double)top) * per, -64000.0);
-    const double big = 6755399441055744.0;  // 1.5 * 2^52
+    const double y = fmax(((double)v - top) * per, -256000.0);
     const double k = y + big;
     const double r = y - (k - big);
-    constexpr double c = 0.6931471805599453 / 64;
-    double p = fma(r, c * c * c * c / 24, c * c * c / 6);
-    p = fma(r, p, c * c / 2);
-    p = fma(r, p, c);
-    p = fma(r, p, 1.0);
-    const int n = (int)__double2loint(k);
-    const double q = power[n & 63];
-    return p * __hiloint2double(__double2hiint(q) + ((n & ~63) << 14),
+    const double p = fma(r, fma(r, fma(r, c3, c2), c1), 1.0);
+    const int n = __double2loint(k);
+    const double q = power[n & 255];
+    return p * __hiloint2double(__double2hiint(q) + ((n & ~255) << 12),
                                 __double2loint(q));
   }
   __device__ __forceinline__ u64 whole(double w) const {
     return (u64)(__double_as_longlong(w + unit) - __double_as_longlong(unit));
   }
+  // of a value that may be infinite, as the largest then is
   __device__ __forceinline__ u64 whole_of(float v) const {
-    return whole(of(v));
+    return whole((double)v == top ? 1.0 : of(v));
   }
 };
 
@@ -265,7 +322,8 @@ __device__ Cut find_cut(Lds& lds, const Row<T>& row, const Weights& weights,
       auto part_over = [&](unsigned t) {
         u64 part = 0;
         row.each([&](float v, int) {
-          if (order_key(v) > t) part += MASS ? weights.whole_of(v) : 1;
+          if (order_key(v) > t)
+            part += MASS ? weights.whole(weights.of(v)) : 1;
         });
         return block_sum(part, lds.wave[0]);
       };
@@ -300,7 +358,7 @@ __device__ Cut find_cut(Lds& lds, const Row<T>& row, const Weights& weights,
       if (v >= low && v <= high) {
         const int bin = bin_of(v);
         atomicAdd(&lds.count[bin], 1u);
-        if (MASS) atomicAdd(&lds.mass[bin], weights.whole_of(v));
+        if (MASS) atomicAdd(&lds.mass[bin], weights.whole(weights.of(v)));
       }
     });
     __syncthreads();
@@ -395,13 +453,66 @@ __device__ Cut find_cut(Lds& lds, const Row<T>& row, const Weights& weights,
   return Cut{low, w ? (limit - above) / w + 1 : (u64)row.vocab, -1};
 }
 
+// Lists the tokens that can be among the first top_k, if they are few: those
+// from about the top_k-th largest of the threads' own maxima up. That many
+// tokens lie there at least; in a row in no particular order not many more.
+template <typename T>
+__device__ Cut list_largest(Lds& lds, const Row<T>& row, float own_high,
+                            float top, unsigned top_k) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  for (int i = tid; i < kBins; i += kThreads) lds.count[i] = 0;
+  if (tid == 0) {
+    lds.listed = 0;
+    lds.low = ~0u;
+    lds.answer[0] = kBins;
+  }
+  const bool some = own_high > -INFINITY;
+  float low = -wave_max(some ? -own_high : -INFINITY);
+  if (lane == 0) lds.extreme[1][wave] = low;
+  __syncthreads();
+  low = -wave_max(-lds.extreme[1][lane & (kWaves - 1)]);
+  const float scale = fminf((kBins - 0.5f) / (top - low), 3e38f);
+  const int bin = min(kBins - 1, max(0, (int)((own_high - low) * scale)));
+  if (some) atomicAdd(&lds.count[bin], 1u);
+  __syncthreads();
+  constexpr int kEach = kBins / kThreads;
+  u64 sum = 0;
+  for (int e = 0; e < kEach; ++e)
+    sum += lds.count[kBins - 1 - (tid * kEach + e)];
+  u64 upto = block_scan(sum, lds.wave[0]);
+  for (int e = 0; e < kEach; ++e) {
+    const int b = kBins - 1 - (tid * kEach + e);
+    const u64 own = lds.count[b];
+    if (upto < top_k && upto + own >= top_k) lds.answer[0] = b;
+    upto += own;
+  }
+  __syncthreads();
+  const int from = (int)lds.answer[0];
+  if (from == kBins) return Cut{-INFINITY, (u64)row.vocab, -1};
+  if (some && bin >= from) atomicMin(&lds.low, order_key(own_high));
+  __syncthreads();
+  const float least = key_value(lds.low);
+  row.each([&](float v, int i) {
+    if (v >= least) {
+      const unsigned at = atomicAdd(&lds.listed, 1u);
+      if (at < kList) lds.list[at] = Token{v, i, 0};
+    }
+  });
+  __syncthreads();
+  const int listed = (int)lds.listed;
+  __syncthreads();
+  return Cut{-INFINITY, (u64)row.vocab, listed <= kList ? listed : -1};
+}
+
 // Draws from the listed tokens: ranks them, filters, and sums the kept ones in
-// the order of their indices. Four threads work for a token.
-__device__ void draw_listed(Lds& lds, const Weights& weights, int listed,
-                            u64 top_k, bool by_mass, bool known, u64 most,
-                            double top_p, double min_p, float uniform,
-                            long* out) {
-  const int tid = threadIdx.x, at = tid >> 2, part = tid & 3;
+// the order of their indices. PARTS threads work for a token.
+template <int PARTS>
+__device__ __forceinline__ void draw_listed(
+    Lds& lds, const Weights& weights, int listed, u64 top_k, bool by_mass,
+    bool known, u64 most, double top_p, double min_p, float uniform,
+    long* out) {
+  const int tid = threadIdx.x, at = tid / PARTS, part = tid % PARTS;
   const bool mine = at < listed;
   Token own{0.f, 0, 0};
   double w = 0.0;
@@ -409,25 +520,30 @@ __device__ void draw_listed(Lds& lds, const Weights& weights, int listed,
     own = lds.list[at];
     w = weights.of(own.v);
     own.weight = weights.whole(w);
+    if (part == 0) lds.list[at].weight = own.weight;
   }
   __syncthreads();
-  if (mine && part == 0) lds.list[at].weight = own.weight;
-  __syncthreads();
-  auto over_parts = [&](auto f) {
-    u64 sum = 0;
-    if (mine)
-      for (int j = part; j < listed; j += 4) sum += f(lds.list[j]);
-    sum += __shfl_xor(sum, 1, WAVE_SIZE);
-    return sum + __shfl_xor(sum, 2, WAVE_SIZE);
+  auto over_parts = [](u64 sum) {
+    for (int o = 1; o < PARTS; o <<= 1) sum += __shfl_xor(sum, o, WAVE_SIZE);
+    return sum;
   };
-  auto before = [&](const Token& t) {
-    return t.v > own.v || (t.v == own.v && t.index < own.index);
-  };
-  const u64 rank = over_parts([&](const Token& t) { return (u64)before(t); });
+  u64 mass = 0;
+  unsigned rank = 0;
+  if (mine) {
+#pragma unroll 4
+    for (int j = part; j < listed; j += PARTS) {
+      const Token t = lds.list[j];
+      const bool before =
+          t.v > own.v || (t.v == own.v && t.index < own.index);
+      rank += before;
+      mass += before ? t.weight : 0;
+    }
+  }
+  for (int o = 1; o < PARTS; o <<= 1)
+    rank += __shfl_xor((int)rank, o, WAVE_SIZE);
   bool keep = mine && rank < top_k;
   if (by_mass) {
-    const u64 mass = over_parts(
-        [&](const Token& t) { return before(t) ? t.weight : 0; });
+    mass = over_parts(mass);
     if (!known) {
       const u64 all =
           block_sum(keep && part == 0 ? own.weight : 0, lds.wave[0]);
@@ -441,9 +557,15 @@ __device__ void draw_listed(Lds& lds, const Weights& weights, int listed,
   const u64 total =
       block_sum(keep && part == 0 ? own.weight : 0, lds.wave[0]);
   const u64 target = floor_u64((double)uniform * (double)total, total - 1);
-  const u64 upto = over_parts([&](const Token& t) {
-    return t.index < own.index ? t.weight : 0;
-  });
+  u64 upto = 0;
+  if (mine) {
+#pragma unroll 4
+    for (int j = part; j < listed; j += PARTS) {
+      const Token t = lds.list[j];
+      upto += t.index < own.index ? t.weight : 0;
+    }
+  }
+  upto = over_parts(upto);
   if (keep && part == 0 && upto <= target && target < upto + own.weight)
     *out = own.index;
 }
@@ -452,7 +574,8 @@ template <typename T>
 __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
   __shared__ Lds lds;
   const long number = blockIdx.x;
-  const int tid = threadIdx.x, V = a.vocab, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, V = a.vocab, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const Row<T> row((const T*)a.logits + number * a.row_stride, V);
 
   double temperature =
@@ -469,51 +592,23 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
   if (top_k <= 0 || top_k > V) top_k = V;
   if (min_p > 1.0) min_p = 1.0;
   const bool by_mass = top_p > 0.0 && top_p < 1.0 && top_k > 1;
-  const bool filtered = by_mass || (top_k > 1 && top_k < V);
+  const bool by_count = top_k > 1 && top_k < V;
 
-  if (tid < 64) lds.power[tid] = kPower[tid];
-  // extremes of the logits above -inf, and how many those are
-  float high = -INFINITY, low = INFINITY;
-  unsigned some = 0;
+  if (tid < 256) lds.power[tid] = kPower[tid >> 2] * kFine[tid & 3];
+  float own_high = -INFINITY;
   bool bad = false;
-  if (filtered) {
-    row.each([&](float v, int) {
-      bad |= v != v;
-      high = fmaxf(high, v);
-      if (v > -INFINITY) {
-        low = fminf(low, v);
-        ++some;
-      }
-    });
-  } else {
-    row.each([&](float v, int) {
-      bad |= v != v;
-      high = fmaxf(high, v);
-    });
-  }
-  if (bad) some = 1u << 31;
-  for (int o = 32; o > 0; o >>= 1) {
-    high = fmaxf(high, __shfl_xor(high, o, WAVE_SIZE));
-    low = fminf(low, __shfl_xor(low, o, WAVE_SIZE));
-    const unsigned other = __shfl_xor((int)some, o, WAVE_SIZE);
-    some = ((some + other) & 0x7fffffffu) | ((some | other) & 0x80000000u);
-  }
-  if (lane == 0) {
-    lds.extreme[0][wave] = high;
-    lds.extreme[1][wave] = low;
-    lds.some[wave] = some;
-  }
+  row.each([&](float v, int) {
+    bad |= v != v;
+    own_high = fmaxf(own_high, v);
+  });
+  // a wave with a NaN says so by one
+  float high = wave_max(__any(bad) ? NAN : own_high);
+  if (__any(bad)) high = NAN;
+  if (lane == 0) lds.extreme[0][wave] = high;
   __syncthreads();
-  high = lds.extreme[0][lane & (kWaves - 1)];
-  low = lds.extreme[1][lane & (kWaves - 1)];
-  some = lds.some[lane & (kWaves - 1)];
-  for (int o = kWaves / 2; o > 0; o >>= 1) {
-    high = fmaxf(high, __shfl_xor(high, o, WAVE_SIZE));
-    low = fminf(low, __shfl_xor(low, o, WAVE_SIZE));
-    const unsigned other = __shfl_xor((int)some, o, WAVE_SIZE);
-    some = ((some + other) & 0x7fffffffu) | ((some | other) & 0x80000000u);
-  }
-  if (some >> 31 || high == -INFINITY) {
+  const float wave_high = lds.extreme[0][lane & (kWaves - 1)];
+  high = wave_max(wave_high);
+  if (__any(wave_high != wave_high) || high == -INFINITY) {
     if (tid == 0) a.out[number] = -1;
     return;
   }
@@ -532,17 +627,32 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
     return;
   }
 
-  const Weights weights{
-      top, 64.0 * 1.4426950408889634 / temperature,
-      __longlong_as_double((long long)(1023 + 52 - a.shift) << 52),
-      lds.power};
+  const Weights weights(top, temperature, a.shift, lds);
   Cut cut{-INFINITY, (u64)V, -1};
   if (top == INFINITY) {  // the others weigh nothing
     cut = Cut{top, (u64)top_k, -1};
-  } else if (filtered) {
-    cut.v = low;  // below come those that weigh nothing
-    if (top_k < (long)some)
-      cut = find_cut<false>(lds, row, weights, low, high, (u64)top_k);
+  } else {
+    if (by_count && top_k <= kList)
+      cut = list_largest(lds, row, own_high, top, (unsigned)top_k);
+    if (cut.listed < 0 && (by_count || by_mass)) {
+      // the least logit above -inf, and how many those are
+      float low = INFINITY;
+      u64 some = 0;
+      row.each([&](float v, int) {
+        if (v > -INFINITY) {
+          low = fminf(low, v);
+          ++some;
+        }
+      });
+      some = block_sum(some, lds.wave[0]);
+      low = -wave_max(-low);
+      if (lane == 0) lds.extreme[1][wave] = low;
+      __syncthreads();
+      low = -wave_max(-lds.extreme[1][lane & (kWaves - 1)]);
+      cut.v = low;  // below come those that weigh nothing
+      if ((u64)top_k < some)
+        cut = find_cut<false>(lds, row, weights, low, high, (u64)top_k);
+    }
   }
   bool known = false;
   u64 most = 0;
@@ -551,7 +661,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
     float next = INFINITY;  // the least logit over the cut
     row.each([&](float v, int) {
       if (v > cut.v) {
-        mass += weights.whole_of(v);
+        mass += weights.whole(weights.of(v));
         next = fminf(next, v);
       }
       equal += v == cut.v;
@@ -565,17 +675,21 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
     if (mass <= most) {
       if (each) cut.ties = min(cut.ties, (most - mass) / each + 1);
     } else {
-      for (int o = 32; o > 0; o >>= 1)
-        next = fminf(next, __shfl_xor(next, o, WAVE_SIZE));
+      next = -wave_max(-next);
+      __syncthreads();
       if (lane == 0) lds.extreme[1][wave] = next;
       __syncthreads();
-      for (int w = 0; w < kWaves; ++w) next = fminf(next, lds.extreme[1][w]);
+      next = -wave_max(-lds.extreme[1][lane & (kWaves - 1)]);
       cut = find_cut<true>(lds, row, weights, next, high, most);
     }
   }
   if (cut.listed >= 0) {
-    draw_listed(lds, weights, cut.listed, (u64)top_k, by_mass, known, most,
-                top_p, min_p, uniform, a.out + number);
+    if (cut.listed <= kThreads / 16)
+      draw_listed<16>(lds, weights, cut.listed, (u64)top_k, by_mass, known,
+                      most, top_p, min_p, uniform, a.out + number);
+    else
+      draw_listed<4>(lds, weights, cut.listed, (u64)top_k, by_mass, known,
+                     most, top_p, min_p, uniform, a.out + number);
     return;
   }
 
@@ -583,11 +697,13 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
     const double w = weights.of(v);
     return w < min_p ? 0 : weights.whole(w);
   };
-  const u64 tie_weight = weigh(cut.v);
+  const u64 tie_weight =
+      cut.v == top ? weights.whole(1.0) : weigh(cut.v);
   // how the kept weights lie over the waves' runs
   u64 sum = 0, equal = 0;
   if (cut.v == -INFINITY && !(min_p > 0.0)) {
-    row.each([&](float v, int) { sum += weights.whole_of(v); });
+    row.each(
+        [&](float v, int) { sum += weights.whole(weights.of(v)); });
   } else {
     row.each([&](float v, int) {
       if (v > cut.v) sum += weigh(v);
@@ -605,23 +721,20 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
   auto kept_ties = [&](u64 before, u64 n) {
     return before >= cut.ties ? 0 : min(n, cut.ties - before);
   };
-  // every wave finds the run with the target, a lane for each run
+  // every wave finds the run with the target, a lane for each run (the lanes
+  // behind the first 16 repeat them)
   const int run = lane & (kWaves - 1);
   const u64 run_ties = lds.wave[1][run];
-  const u64 ties_before = wave_scan(lane < kWaves ? run_ties : 0, kWaves) -
-                          (lane < kWaves ? run_ties : 0);
+  const u64 ties_before = wave_scan<true>(run_ties) - run_ties;
   const u64 own =
-      lane < kWaves
-          ? lds.wave[0][run] + kept_ties(ties_before, run_ties) * tie_weight
-          : 0;
-  const u64 run_upto = wave_scan(own, kWaves);
-  const u64 total = __shfl(run_upto, kWaves - 1, WAVE_SIZE);
+      lds.wave[0][run] + kept_ties(ties_before, run_ties) * tie_weight;
+  const u64 run_upto = wave_scan<true>(own);
+  const u64 total = lane_value(run_upto, kWaves - 1);
   const u64 target =
       floor_u64((double)uniform * (double)total, total - 1);
-  const int owner =
-      __builtin_ctzl(__ballot(lane < kWaves && target < run_upto));
-  u64 upto = __shfl(run_upto - own, owner, WAVE_SIZE);
-  const u64 ties = __shfl(ties_before, owner, WAVE_SIZE);
+  const int owner = __builtin_ctzl(__ballot(target < run_upto));
+  u64 upto = lane_value(run_upto - own, owner);
+  const u64 ties = lane_value(ties_before, owner);
   // all threads share that run, each a few neighbours
   if (tid == owner * 64) {
     lds.answer[0] = row.first;
