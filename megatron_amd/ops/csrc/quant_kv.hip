@@ -68,11 +68,16 @@ __device__ __forceinline__ long v_meta_at(const CacheView& c, long bh, long t,
   return ((bh * (c.h / kGroup) + group) * (c.room / 4) + t / 4) * 8 + (t & 3);
 }
 
-// code of x: the nearest whole number of s above z, ties to even. The quotient
-// in 32 bits is off by less than one code; 64-bit products decide.
+// code of x: the nearest whole number of s above z, ties to even. In 32 bits
+// the quotient is off by 16 * 3 * 2^-24 where it is up to 16; nearer to a
+// border than three times that, products in 64 bits decide.
 __device__ __forceinline__ unsigned code_of(float x, float z, float s,
                                             float inv) {
   if (!(s > 0.f)) return 0;
+  const float q = (x - z) * inv;
+  const float whole = rintf(q);
+  if (fabsf(fabsf(q - whole) - 0.5f) > 1e-5f)
+    return (unsigned)fminf(fmaxf(whole, 0.f), 15.f);
   const double above = (double)x - (double)z;
   float n = floorf((float)above * inv);
   n = fminf(fmaxf(n, 0.f), 15.f);
@@ -123,165 +128,323 @@ __device__ __forceinline__ float rotated(const T* x, const float* cos_row,
   return DTypeTraits<T>::to_float(DTypeTraits<T>::from_float(to_32(y)));
 }
 
-// A row (token, sequence, head) takes h / 8 lanes with 8 values each; four
-// lanes share a group. Rows of q, if any, come behind those of k and v and
-// are only rotated.
 template <typename T>
-__global__ __launch_bounds__(256) void append_kernel(
+union Eight {
+  uint4 u;
+  T t[8];
+};
+
+template <typename T>
+__device__ __forceinline__ void load_eight(float (&y)[8], const T* x,
+                                           bool wide) {
+  Eight<T> v;
+  if (wide) {
+    v.u = *(const uint4*)x;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v.t[i] = x[i];
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] = DTypeTraits<T>::to_float(v.t[i]);
+}
+
+// Four lanes hold a group's 32 values: codes in the order of the values from
+// the lowest bits up, and its scale and zero point. A NaN counts as 0.
+struct Held {
+  unsigned code[8];
+  __half scale, zero;
+  bool nan;  // in the group
+};
+
+__device__ __forceinline__ Held hold_eight(const float (&x)[8]) {
+  Held y;
+  float v[8], low = INFINITY, high = -INFINITY;
+  int nan = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    nan |= x[i] != x[i];
+    v[i] = x[i] != x[i] ? 0.f : fminf(fmaxf(x[i], -kHeldMax), kHeldMax);
+    low = fminf(low, v[i]);
+    high = fmaxf(high, v[i]);
+  }
+#pragma unroll
+  for (int o = 1; o < 4; o <<= 1) {
+    low = fminf(low, __shfl_xor(low, o, WAVE_SIZE));
+    high = fmaxf(high, __shfl_xor(high, o, WAVE_SIZE));
+    nan |= __shfl_xor(nan, o, WAVE_SIZE);
+  }
+  y.nan = nan;
+  y.zero = __float2half(low);
+  const float z = __half2float(y.zero);
+  y.scale = __float2half(to_32(((double)high - (double)z) / 15.0));
+  const float s = __half2float(y.scale), inv = 1.f / s;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y.code[i] = code_of(v[i], z, s, inv);
+  return y;
+}
+
+// Codes of a key's word and of a value's, in the cache's order.
+__device__ __forceinline__ unsigned key_word(const Held& y) {
+  unsigned w = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w |= y.code[i] << ((i >> 1) * 4 + (i & 1) * 16);
+  return w;
+}
+
+__device__ __forceinline__ unsigned value_word(const Held& y) {
+  unsigned w = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w |= y.code[i] << (i * 4);
+  return w;
+}
+
+__device__ __forceinline__ int row_any(int v, int lanes) {
+  for (int o = 1; o < lanes; o <<= 1) v |= __shfl_xor(v, o, WAVE_SIZE);
+  return v;
+}
+
+// The scales and zero points of a row's groups, by the first lane of each.
+__device__ __forceinline__ void store_scales(const CacheView& cache, long bh,
+                                             long pos, int part,
+                                             const Held& k, const Held& v,
+                                             bool nan_row) {
+  if (part & 3) return;
+  const __half nan = __ushort_as_half(0x7e00);
+  const int group = part / 4;
+  const __half2 m = {nan_row ? nan : k.scale, k.zero};
+  ((__half2*)cache.k_meta)[(bh * cache.room + pos) * (cache.h / kGroup) +
+                           group] = m;
+  __half* w = cache.v_meta + v_meta_at(cache, bh, pos, group);
+  w[0] = v.nan ? nan : v.scale;
+  w[4] = v.zero;
+}
+
+// A prompt: a wave takes 512 / h neighbouring positions of one head, aligned
+// to as many, h / 8 lanes and 8 values a lane for each, so that the pairs of
+// tokens that share words of v_codes meet in a wave and all stores are whole
+// words next to each other.
+template <typename T>
+__global__ __launch_bounds__(256) void append_kernel(CacheView cache,
+                                                     AppendSource k,
+                                                     AppendSource v, bool wide,
+                                                     Start start, long s,
+                                                     long tiles) {
+  const int lanes = cache.h / 8, per = 64 / lanes;
+  const int lane = threadIdx.x & 63;
+  const int part = lane & (lanes - 1), d0 = part * 8;
+  const long wave =
+      (long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const long bh = wave / tiles;
+  if (bh >= (long)cache.b * cache.heads) return;
+  const int ib = (unsigned)bh / (unsigned)cache.heads;
+  const int head = (int)bh - ib * cache.heads;
+  const long t = start.of(ib);
+  if (t < 0) return;  // idle
+  // positions from the begin's tile on
+  const long pos = (t / per + (wave - bh * tiles)) * per + lane / lanes;
+  const long is = pos - t;
+  const bool real = is >= 0 && is < s && pos < cache.capacity;
+  float kx[8] = {}, vx[8] = {};
+  if (real) {
+    load_eight((float(&)[8])kx,
+               (const T*)k.x + is * k.ss + ib * k.bs + head * k.ns + d0, wide);
+    load_eight((float(&)[8])vx,
+               (const T*)v.x + is * v.ss + ib * v.bs + head * v.ns + d0, wide);
+  }
+  const Held hk = hold_eight(kx), hv = hold_eight(vx);
+  const bool nan_row = row_any(hk.nan || hv.nan, lanes);
+
+  if (real) {
+    ((unsigned*)cache.k_codes)[(bh * cache.room + pos) * (cache.h / 8) +
+                               part] = key_word(hk);
+    store_scales(cache, bh, pos, part, hk, hv, nan_row);
+  }
+  const unsigned own = value_word(hv);
+  const unsigned other = __shfl_xor(own, lanes, WAVE_SIZE);
+  const int other_real = __shfl_xor((int)real, lanes, WAVE_SIZE);
+  const bool both = real && other_real;
+  unsigned short* pieces = (unsigned short*)cache.v_codes;
+  if (cache.h < 64) {  // a piece has two values
+    if (real)
+      for (int i = 0; i < 4; ++i)
+        pieces[v_piece(cache, bh, pos, d0 + 2 * i)] = (own >> (8 * i)) & 255;
+  } else if (both) {  // one word of two pieces for either token's lane
+    const bool odd = pos & 1;
+    const unsigned word = odd ? (other >> 16) | (own & 0xffff0000u)
+                              : (own & 0xffffu) | (other << 16);
+    const long at = v_piece(cache, bh, pos & ~1l, d0 + (odd ? 4 : 0));
+    *(unsigned*)(pieces + at) = word;
+  } else if (real) {
+    pieces[v_piece(cache, bh, pos, d0)] = (unsigned short)own;
+    pieces[v_piece(cache, bh, pos, d0 + 4)] = (unsigned short)(own >> 16);
+  }
+}
+
+// A decode step: a row (token, sequence, head) takes h / 8 lanes with 8 values
+// each. Rows of q come behind those of k and v and are only rotated.
+template <typename T>
+__global__ __launch_bounds__(256) void append_rotated_kernel(
     CacheView cache, AppendSource k, AppendSource v, AppendSource q,
     T* __restrict__ q_out, int n, const float* __restrict__ cos_t,
     const float* __restrict__ sin_t, int r, long table_rows, bool interleaved,
-    Start start, long s) {
+    bool wide, Start start, long s) {
   const int lanes = cache.h / 8;
-  const long index = (long)blockIdx.x * 256 + threadIdx.x;
-  const long row = index / lanes;
-  const int part = index % lanes, d0 = part * 8;
-  const long kv_rows = s * cache.b * cache.heads;
-  const long rows = kv_rows + (q.x ? s * cache.b * n : 0);
+  const unsigned index = blockIdx.x * 256 + threadIdx.x;
+  const unsigned row = index / (unsigned)lanes;
+  const int part = index & (lanes - 1), d0 = part * 8;
+  const unsigned kv_rows = (unsigned)s * cache.b * cache.heads;
+  const unsigned rows = kv_rows + (unsigned)s * cache.b * n;
   if (row >= rows) return;
   const bool is_q = row >= kv_rows;
-  const int heads = is_q ? n : cache.heads;
-  const long local = is_q ? row - kv_rows : row;
-  const int head = local % heads;
-  const int ib = (local / heads) % cache.b;
-  const long is = local / heads / cache.b;
+  const unsigned heads = is_q ? n : cache.heads;
+  const unsigned local = is_q ? row - kv_rows : row;
+  const unsigned token = local / heads;
+  const int head = local - token * heads;
+  const int is = token / (unsigned)cache.b;
+  const int ib = token - is * cache.b;
+  const AppendSource& from = is_q ? q : k;
+  const T* x =
+      (const T*)from.x + is * from.ss + ib * from.bs + head * from.ns;
+  float own[8], vx[8], pair[8], c[8], sn[8];
+  load_eight(own, x + d0, wide);
+  if (!is_q)
+    load_eight(vx,
+               (const T*)v.x + is * v.ss + ib * v.bs + head * v.ns + d0, wide);
   const long t = start.of(ib);
   const bool idle = t < 0;
   const long pos = t + is;
+  const bool known = !idle && pos < table_rows;
 
-  const float *cos_row = nullptr, *sin_row = nullptr;
-  const bool turn = r > 0;
-  const bool known = pos >= 0 && pos < table_rows;
-  if (turn && known) {
-    cos_row = cos_t + pos * r;
-    sin_row = sin_t + pos * r;
+  // Rotation in 64 bits, rounded to T: the codes of a rotated key hang on it.
+  // A lane's values lie before or behind their partners, or are a pair's both.
+  const bool turns = d0 < 2 * r;
+  if (turns && known) {
+    const float* cos_row = cos_t + pos * r;
+    const float* sin_row = sin_t + pos * r;
+    if (interleaved || r % 8 == 0) {
+      const bool behind = !interleaved && d0 >= r;
+      const int j0 = interleaved ? d0 / 2 : behind ? d0 - r : d0;
+      const int turned = interleaved ? 4 : 8;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < turned && j0 + i < r) {
+          c[i] = cos_row[j0 + i];
+          sn[i] = sin_row[j0 + i];
+        }
+      if (interleaved) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (j0 + i >= r) break;
+          const double x1 = own[2 * i], x2 = own[2 * i + 1];
+          const double y1 = x1 * c[i] - x2 * sn[i];
+          const double y2 = x2 * c[i] + x1 * sn[i];
+          own[2 * i] = to_32(y1);
+          own[2 * i + 1] = to_32(y2);
+        }
+      } else {
+        load_eight(pair, x + (behind ? d0 - r : d0 + r), wide);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const double a = (double)own[i] * c[i];
+          const double b = (double)pair[i] * sn[i];
+          own[i] = to_32(behind ? a + b : a - b);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        own[i] = DTypeTraits<T>::to_float(DTypeTraits<T>::from_float(own[i]));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        own[i] = rotated<T>(x, cos_row, sin_row, d0 + i, r, interleaved);
+    }
+  } else if (turns) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (d0 + i < 2 * r) own[i] = NAN;
   }
-  auto value = [&](const T* x, int d) -> float {
-    if (!turn) return DTypeTraits<T>::to_float(x[d]);
-    if (!known && d < 2 * r) return NAN;
-    return rotated<T>(x, cos_row, sin_row, d, r, interleaved);
-  };
 
   if (is_q) {
-    const T* x = (const T*)q.x + is * q.ss + ib * q.bs + head * q.ns;
-    T* y = q_out + local * cache.h + d0;
+    Eight<T> y;
+#pragma unroll
     for (int i = 0; i < 8; ++i)
-      y[i] = DTypeTraits<T>::from_float(idle ? 0.f : value(x, d0 + i));
+      y.t[i] = DTypeTraits<T>::from_float(idle ? 0.f : own[i]);
+    *(uint4*)(q_out + (long)local * cache.h + d0) = y.u;
     return;
   }
-  if (idle || pos >= cache.capacity) return;  // a whole row returns together
-
-  const T* kx = (const T*)k.x + is * k.ss + ib * k.bs + head * k.ns;
-  const T* vx = (const T*)v.x + is * v.ss + ib * v.bs + head * v.ns;
-  float kv[8], vv[8];
-  bool nan_k = false, nan_v = false;
-  float k_low = INFINITY, k_high = -INFINITY;
-  float v_low = INFINITY, v_high = -INFINITY;
-  for (int i = 0; i < 8; ++i) {
-    const float a = value(kx, d0 + i);
-    const float b = DTypeTraits<T>::to_float(vx[d0 + i]);
-    nan_k |= a != a;
-    nan_v |= b != b;
-    kv[i] = a != a ? 0.f : fminf(fmaxf(a, -kHeldMax), kHeldMax);
-    vv[i] = b != b ? 0.f : fminf(fmaxf(b, -kHeldMax), kHeldMax);
-    k_low = fminf(k_low, kv[i]);
-    k_high = fmaxf(k_high, kv[i]);
-    v_low = fminf(v_low, vv[i]);
-    v_high = fmaxf(v_high, vv[i]);
-  }
-  // lanes of a row share a wave: 64 is a multiple of h / 8
-  for (int o = 1; o < 4; o <<= 1) {
-    k_low = fminf(k_low, __shfl_xor(k_low, o, WAVE_SIZE));
-    k_high = fmaxf(k_high, __shfl_xor(k_high, o, WAVE_SIZE));
-    v_low = fminf(v_low, __shfl_xor(v_low, o, WAVE_SIZE));
-    v_high = fmaxf(v_high, __shfl_xor(v_high, o, WAVE_SIZE));
-  }
-  int nan_group = nan_v, nan_row = nan_k || nan_v;
-  for (int o = 1; o < 4; o <<= 1)
-    nan_group |= __shfl_xor(nan_group, o, WAVE_SIZE);
-  for (int o = 1; o < lanes; o <<= 1)
-    nan_row |= __shfl_xor(nan_row, o, WAVE_SIZE);
-
-  const __half k_z = __float2half(k_low), v_z = __float2half(v_low);
-  const float kz = __half2float(k_z), vz = __half2float(v_z);
-  __half k_s = __float2half(to_32(((double)k_high - (double)kz) / 15.0));
-  __half v_s = __float2half(to_32(((double)v_high - (double)vz) / 15.0));
-  const float ks = __half2float(k_s), vs = __half2float(v_s);
-  const float k_inv = 1.f / ks, v_inv = 1.f / vs;
-  unsigned k_word = 0, v_word = 0;
-  for (int i = 0; i < 8; ++i) {
-    k_word |= code_of(kv[i], kz, ks, k_inv) << ((i >> 1) * 4 + (i & 1) * 16);
-    v_word |= code_of(vv[i], vz, vs, v_inv) << (i * 4);
-  }
-  const __half nan = __ushort_as_half(0x7e00);
-  if (nan_row) k_s = nan;
-  if (nan_group) v_s = nan;
-
+  const bool real = !idle && pos < cache.capacity;  // of the whole row
+  const Held hk = hold_eight(own), hv = hold_eight(vx);
+  const bool nan_row = row_any(hk.nan || hv.nan, lanes);
+  if (!real) return;
   const long bh = (long)ib * cache.heads + head;
-  const long tok = bh * cache.room + pos;
-  *(unsigned*)(cache.k_codes + tok * (cache.h / 2) + part * 4) = k_word;
+  ((unsigned*)cache.k_codes)[(bh * cache.room + pos) * (cache.h / 8) + part] =
+      key_word(hk);
+  store_scales(cache, bh, pos, part, hk, hv, nan_row);
+  const unsigned word = value_word(hv);
   unsigned short* pieces = (unsigned short*)cache.v_codes;
   if (cache.h >= 64) {
-    pieces[v_piece(cache, bh, pos, d0)] = (unsigned short)v_word;
-    pieces[v_piece(cache, bh, pos, d0 + 4)] = (unsigned short)(v_word >> 16);
+    pieces[v_piece(cache, bh, pos, d0)] = (unsigned short)word;
+    pieces[v_piece(cache, bh, pos, d0 + 4)] = (unsigned short)(word >> 16);
   } else {  // a piece has two values
     for (int i = 0; i < 4; ++i)
-      pieces[v_piece(cache, bh, pos, d0 + 2 * i)] = (v_word >> (8 * i)) & 255;
-  }
-  if ((part & 3) == 0) {
-    const int group = part / 4;
-    __half* m = cache.k_meta + (tok * (cache.h / kGroup) + group) * 2;
-    m[0] = k_s;
-    m[1] = k_z;
-    __half* w = cache.v_meta + v_meta_at(cache, bh, pos, group);
-    w[0] = v_s;
-    w[4] = v_z;
+      pieces[v_piece(cache, bh, pos, d0 + 2 * i)] = (word >> (8 * i)) & 255;
   }
 }
 
-__device__ __forceinline__ float held_k(const CacheView& c, long bh, long t,
-                                        int d) {
-  const long tok = bh * c.room + t;
-  const unsigned word =
-      *(const unsigned*)(c.k_codes + tok * (c.h / 2) + d / 8 * 4);
-  const int i = d & 7;
-  const float code = (word >> ((i >> 1) * 4 + (i & 1) * 16)) & 15;
-  const __half* m = c.k_meta + (tok * (c.h / kGroup) + d / kGroup) * 2;
-  return __half2float(m[1]) + __half2float(m[0]) * code;
-}
-
-__device__ __forceinline__ float held_v(const CacheView& c, long bh, long t,
-                                        int d) {
-  const unsigned piece =
-      ((const unsigned short*)c.v_codes)[v_piece(c, bh, t, d)];
-  const int within = c.h >= 64 ? d % 4 : d % 2;
-  const float code = (piece >> (within * 4)) & 15;
-  const __half* m = c.v_meta + v_meta_at(c, bh, t, d / kGroup);
-  return __half2float(m[4]) + __half2float(m[0]) * code;
-}
-
-// One thread per value; positions outside the cache read as NaN.
+// Reads back with the same lanes as append_kernel; positions outside the cache
+// read as NaN.
 template <typename T>
 __global__ __launch_bounds__(256) void dequantize_kernel(
-    CacheView cache, Start start, long length, T* __restrict__ k_out,
-    T* __restrict__ v_out) {
-  const long total = length * cache.b * cache.heads * cache.h;
-  for (long idx = (long)blockIdx.x * 256 + threadIdx.x; idx < total;
-       idx += (long)gridDim.x * 256) {
-    const int d = idx % cache.h;
-    const long row = idx / cache.h;
-    const int head = row % cache.heads;
-    const int ib = (row / cache.heads) % cache.b;
-    const long pos = start.of(ib) + row / cache.heads / cache.b;
-    float k = NAN, v = NAN;
-    if (pos >= 0 && pos < cache.capacity) {
-      const long bh = (long)ib * cache.heads + head;
-      k = held_k(cache, bh, pos, d);
-      v = held_v(cache, bh, pos, d);
+    CacheView cache, Start start, long length, long tiles,
+    T* __restrict__ k_out, T* __restrict__ v_out) {
+  const int lanes = cache.h / 8, per = 64 / lanes;
+  const int lane = threadIdx.x & 63;
+  const int part = lane & (lanes - 1), d0 = part * 8;
+  const long wave =
+      (long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const long bh = wave / tiles;
+  if (bh >= (long)cache.b * cache.heads) return;
+  const int ib = (unsigned)bh / (unsigned)cache.heads;
+  const int head = (int)bh - ib * cache.heads;
+  const long t = start.of(ib);
+  // positions from the begin's tile on, rounded down also where it is negative
+  const long tile = (t >= 0 ? t / per : -((per - 1 - t) / per));
+  const long pos = (tile + (wave - bh * tiles)) * per + lane / lanes;
+  const long is = pos - t;
+  if (is < 0 || is >= length) return;
+  Eight<T> ky, vy;
+  if (pos >= 0 && pos < cache.capacity) {
+    const int groups = cache.h / kGroup, group = part / 4;
+    const long tok = bh * cache.room + pos;
+    const unsigned kw = ((const unsigned*)cache.k_codes)[tok * lanes + part];
+    const __half2 km = ((const __half2*)cache.k_meta)[tok * groups + group];
+    const unsigned short* pieces = (const unsigned short*)cache.v_codes;
+    unsigned vw = 0;
+    if (cache.h >= 64) {
+      vw = pieces[v_piece(cache, bh, pos, d0)] |
+           (unsigned)pieces[v_piece(cache, bh, pos, d0 + 4)] << 16;
+    } else {
+      for (int i = 0; i < 4; ++i)
+        vw |= (pieces[v_piece(cache, bh, pos, d0 + 2 * i)] & 255u) << (8 * i);
     }
-    k_out[idx] = DTypeTraits<T>::from_float(k);
-    v_out[idx] = DTypeTraits<T>::from_float(v);
+    const __half* vm = cache.v_meta + v_meta_at(cache, bh, pos, group);
+    const float ks = __half2float(km.x), kz = __half2float(km.y);
+    const float vs = __half2float(vm[0]), vz = __half2float(vm[4]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      ky.t[i] = DTypeTraits<T>::from_float(
+          fmaf(ks, (float)((kw >> ((i >> 1) * 4 + (i & 1) * 16)) & 15), kz));
+      vy.t[i] = DTypeTraits<T>::from_float(
+          fmaf(vs, (float)((vw >> (i * 4)) & 15), vz));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      ky.t[i] = vy.t[i] = DTypeTraits<T>::from_float(NAN);
   }
+  const long at = ((is * cache.b + ib) * cache.heads + head) * cache.h + d0;
+  *(uint4*)(k_out + at) = ky.u;
+  *(uint4*)(v_out + at) = vy.u;
 }
 
 // ---------------------------------------------------------------------------
@@ -1133,16 +1296,34 @@ c10::optional<torch::Tensor> quant_kv_append(
     TORCH_CHECK(!query.has_value() && !sin.has_value(),
                 "quant_kv: query, cos and sin come together");
   }
-  const long rows = s * cache.b * (cache.heads + (long)n);
-  if (rows > 0) {
-    const long grid = (rows * (cache.h / 8) + 255) / 256;
+  auto wide = [](const torch::Tensor& x) {
+    return (unsigned long)x.data_ptr() % 16 == 0 && x.stride(0) % 8 == 0 &&
+           x.stride(1) % 8 == 0 && x.stride(2) % 8 == 0;
+  };
+  bool all_wide = wide(key) && wide(value);
+  auto stream = c10::hip::getCurrentHIPStream();
+  if (s > 0 && q.x) {
+    all_wide = all_wide && wide(*query);
+    const long grid =
+        (s * cache.b * (cache.heads + (long)n) * (cache.h / 8) + 255) / 256;
+    TORCH_CHECK(grid < (1l << 24), "quant_kv: too many tokens at once");
+#define LAUNCH_APPEND(T)                                                     \
+  hipLaunchKernelGGL((append_rotated_kernel<T>), dim3(grid), dim3(256), 0,   \
+                     stream, cache, source_of(key), source_of(value), q,     \
+                     (T*)q_out.data_ptr(), n, cos_p, sin_p, r, table_rows,   \
+                     interleaved, all_wide, at, s)
+    DISPATCH_HALF(key, LAUNCH_APPEND);
+#undef LAUNCH_APPEND
+    HIP_CHECK(hipGetLastError());
+  } else if (s > 0) {
+    // the begin may lie anywhere in a wave's tile
+    const long per = 512 / cache.h, tiles = (s + per - 2) / per + 1;
+    const long grid = ((long)cache.b * cache.heads * tiles + 3) / 4;
     TORCH_CHECK(grid < (1l << 31), "quant_kv: too many tokens at once");
-    auto stream = c10::hip::getCurrentHIPStream();
 #define LAUNCH_APPEND(T)                                                     \
   hipLaunchKernelGGL((append_kernel<T>), dim3(grid), dim3(256), 0, stream,   \
-                     cache, source_of(key), source_of(value), q,             \
-                     q.x ? (T*)q_out.data_ptr() : nullptr, n, cos_p, sin_p,  \
-                     r, table_rows, interleaved, at, s)
+                     cache, source_of(key), source_of(value), all_wide, at,  \
+                     s, tiles)
     DISPATCH_HALF(key, LAUNCH_APPEND);
 #undef LAUNCH_APPEND
     HIP_CHECK(hipGetLastError());
@@ -1163,12 +1344,14 @@ std::vector<torch::Tensor> quant_kv_dequantize(
   auto k = torch::empty({length, cache.b, cache.heads, cache.h}, options);
   auto v = torch::empty_like(k);
   if (k.numel() == 0) return {k, v};
-  const int grid = (int)std::min<long>((k.numel() + 255) / 256, 32768);
+  const long per = 512 / cache.h, tiles = (length + per - 2) / per + 1;
+  const long grid = ((long)cache.b * cache.heads * tiles + 3) / 4;
+  TORCH_CHECK(grid < (1l << 31), "quant_kv: too many tokens at once");
   auto stream = c10::hip::getCurrentHIPStream();
 #define LAUNCH_DEQUANTIZE(T)                                                 \
   hipLaunchKernelGGL((dequantize_kernel<T>), dim3(grid), dim3(256), 0,       \
-                     stream, cache, at, (long)length, (T*)k.data_ptr(),      \
-                     (T*)v.data_ptr())
+                     stream, cache, at, (long)length, tiles,                 \
+                     (T*)k.data_ptr(), (T*)v.data_ptr())
   DISPATCH_HALF(k, LAUNCH_DEQUANTIZE);
 #undef LAUNCH_DEQUANTIZE
   HIP_CHECK(hipGetLastError());

@@ -588,7 +588,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
     temperature = 1.0;
     top_k = 1;
   }
-  temperature = fmin(temperature, 1e30);
+  temperature = fmin(fmax(temperature, 1e-300), 1e30);
   if (top_k <= 0 || top_k > V) top_k = V;
   if (min_p > 1.0) min_p = 1.0;
   const bool by_mass = top_p > 0.0 && top_p < 1.0 && top_k > 1;
