@@ -274,7 +274,8 @@ def load_args_from_checkpoint(cfg):
         "make_vocab_size_divisible_by", "padded_vocab_size", "use_bias",
         "use_rms_norm", "use_post_ln", "glu_activation",
         "position_embedding_type", "rope_theta", "rope_scaling_factor",
-        "tie_embed_logits", "parallel_attn", "parallel_layernorm",
+        "rope_scaling_type", "rope_original_max_positions", "rotary_layout",
+        "rotary_percent", "tie_embed_logits", "parallel_attn", "parallel_layernorm",
         "sliding_window_size", "layernorm_epsilon", "tokenizer_type",
     ):
         if hasattr(checkpoint_args, key):

@@ -39,6 +39,12 @@ class TrainingConfig:
     position_embedding_type: str = "absolute"  # 'absolute' | 'rotary'
     rope_theta: float = 10000.0
     rope_scaling_factor: float = 1.0
+    # how a context longer than the trained one is reached by
+    # rope_scaling_factor: 'linear' | 'ntk' | 'yarn' (models/rope.py)
+    rope_scaling_type: str = "linear"
+    rope_original_max_positions: Optional[int] = None  # yarn: trained length
+    rotary_layout: str = "interleaved"  # pairs: 'interleaved' | 'half'
+    rotary_percent: float = 1.0         # part of the head that is rotated
     tie_embed_logits: bool = True       # tie lm head to word embeddings
     parallel_attn: bool = False         # Falcon parallel attention+MLP
     parallel_layernorm: bool = False    # Falcon-40B separate ln_mlp
@@ -255,6 +261,11 @@ class TrainingConfig:
 
     # -- inference --
     inference_batch_times_seqlen_threshold: int = 512
+    # 4: keys and values of generation are held in 4 bits (ops/quant_kv.py);
+    # attention_sink_size then keeps that many first tokens visible besides
+    # the sliding window
+    kv_cache_bits: int = 16
+    attention_sink_size: int = 0
     max_tokens_to_oom: int = 12000
 
     # -- misc --
@@ -361,6 +372,24 @@ class TrainingConfig:
 
         if self.recompute_granularity == "full":
             assert self.recompute_method in ("uniform", "block", None)
+
+        assert self.rope_scaling_type in ("linear", "ntk", "yarn")
+        assert self.rotary_layout in ("interleaved", "half")
+        assert 0.0 < self.rotary_percent <= 1.0
+        if self.rope_scaling_type == "yarn":
+            assert self.rope_original_max_positions is not None, (
+                "yarn needs rope_original_max_positions"
+            )
+        assert self.kv_cache_bits in (4, 16), "kv_cache_bits is 4 or 16"
+        if self.attention_sink_size:
+            assert self.kv_cache_bits == 4 and self.sliding_window_size, (
+                "attention_sink_size needs kv_cache_bits 4 and a sliding "
+                "window"
+            )
+        if self.kv_cache_bits == 4:
+            assert self.pipeline_model_parallel_size == 1, (
+                "kv_cache_bits 4 needs pipeline_model_parallel_size 1"
+            )
 
         if self.lr_warmup_fraction is not None:
             assert self.lr_warmup_iters == 0 and self.lr_warmup_samples == 0

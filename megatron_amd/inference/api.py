@@ -20,6 +20,7 @@ def generate_and_post_process(
     top_k_sampling=0, top_p_sampling=0.0, temperature=1.0, add_BOS=False,
     use_eod_token_for_early_termination=True, stop_on_double_eol=False,
     stop_on_eol=False, prevent_newline_after_colon=False, random_seed=-1,
+    min_p_sampling=0.0,
 ):
     """(reference api.py:19-66)"""
     tokens, lengths, output_log_probs = generate(
@@ -30,7 +31,7 @@ def generate_and_post_process(
         use_eod_token_for_early_termination=use_eod_token_for_early_termination,
         stop_on_double_eol=stop_on_double_eol, stop_on_eol=stop_on_eol,
         prevent_newline_after_colon=prevent_newline_after_colon,
-        random_seed=random_seed,
+        random_seed=random_seed, min_p_sampling=min_p_sampling,
     )
     if mpu.is_pipeline_first_stage() and mpu.get_tensor_model_parallel_rank() == 0:
         tokens, prompts_plus_generations, segments = detokenize_generations(
@@ -49,13 +50,14 @@ def generate(model, prompts=None, tokens_to_generate=0,
              top_p_sampling=0.0, temperature=1.0, add_BOS=False,
              use_eod_token_for_early_termination=True,
              stop_on_double_eol=False, stop_on_eol=False,
-             prevent_newline_after_colon=False, random_seed=-1):
+             prevent_newline_after_colon=False, random_seed=-1,
+             min_p_sampling=0.0):
     """(reference api.py:70-135)"""
     values = [
         tokens_to_generate, return_output_log_probs, top_k_sampling,
         top_p_sampling, temperature, add_BOS,
         use_eod_token_for_early_termination, stop_on_double_eol, stop_on_eol,
-        prevent_newline_after_colon, random_seed,
+        prevent_newline_after_colon, random_seed, min_p_sampling,
     ]
     values_float_tensor = broadcast_float_list(
         len(values), float_list=values
@@ -71,6 +73,7 @@ def generate(model, prompts=None, tokens_to_generate=0,
     stop_on_eol = bool(values_float_tensor[8].item())
     prevent_newline_after_colon = bool(values_float_tensor[9].item())
     random_seed = int(values_float_tensor[10].item())
+    min_p_sampling = values_float_tensor[11].item()
 
     if random_seed != -1:
         torch.random.manual_seed(random_seed)
@@ -91,6 +94,7 @@ def generate(model, prompts=None, tokens_to_generate=0,
         use_eod_token_for_early_termination=use_eod_token_for_early_termination,
         stop_on_double_eol=stop_on_double_eol, stop_on_eol=stop_on_eol,
         prevent_newline_after_colon=prevent_newline_after_colon,
+        min_p=min_p_sampling,
     )
 
 

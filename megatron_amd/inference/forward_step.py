@@ -7,6 +7,7 @@ import torch
 
 from .. import parallel as mpu
 from ..config import get_config
+from ..ops import QuantKVCache
 from .communication import (
     recv_from_prev_pipeline_rank_,
     send_to_next_pipeline_rank,
@@ -27,6 +28,10 @@ class InferenceParams:
         if len(self.key_value_memory_dict) == 0:
             raise ValueError("should not swap when dict in empty")
         for layer_number in self.key_value_memory_dict.keys():
+            if isinstance(self.key_value_memory_dict[layer_number],
+                          QuantKVCache):
+                self.key_value_memory_dict[layer_number].reorder(batch_idx)
+                continue
             inference_key_memory, inference_value_memory = (
                 self.key_value_memory_dict[layer_number]
             )

@@ -64,7 +64,7 @@ def generate_tokens_probs_and_return_on_first_stage(
     model, tokens, lengths, return_output_log_probs=False,
     top_k=0, top_p=0.0, temperature=1.0, use_eod_token_for_early_termination=True,
     stop_on_double_eol=False, stop_on_eol=False, prevent_newline_after_colon=False,
-    echo_prompts=False,
+    echo_prompts=False, min_p=0.0,
 ):
     """Main generation loop (reference generation.py:89-285)."""
     cfg = get_config()
@@ -129,6 +129,7 @@ def generate_tokens_probs_and_return_on_first_stage(
                     last_token_logits.float(), top_k=top_k, top_p=top_p,
                     temperature=temperature,
                     vocab_size=getattr(tokenizer, "vocab_size", None),
+                    min_p=min_p,
                 )
                 # only update tokens past each prompt
                 started = lengths <= context_length

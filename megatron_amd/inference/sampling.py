@@ -1,9 +1,12 @@
 """Token sampling: greedy / top-k / top-p with temperature
-(reference megatron/text_generation/sampling.py:18-98)."""
+(reference megatron/text_generation/sampling.py:18-98), and, with min-p or given
+uniform numbers, all filters at once in one kernel (ops.sample_tokens)."""
 
 from __future__ import annotations
 
 import torch
+
+from ..ops import sample_tokens
 
 
 def modify_logits_for_top_k_filtering(logits, top_k):
@@ -22,10 +25,25 @@ def modify_logits_for_top_p_filtering(logits, top_p):
     logits.masked_fill_(filter_, float("-inf"))
 
 
-def sample(logits, top_k=0, top_p=0.0, temperature=1.0, vocab_size=None):
+def sample(logits, top_k=0, top_p=0.0, temperature=1.0, vocab_size=None,
+           min_p=0.0, uniform=None):
     """Sample one token per row of logits [b, v]
-    (reference sampling.py:45-98)."""
+    (reference sampling.py:45-98).
+
+    With min_p > 0 or uniform (float32 [b] in [0, 1)) the filters combine as in
+    ops.sample_tokens, tokens at or past vocab_size are never drawn, and
+    uniform defaults to torch.rand. A row that leaves nothing to draw from
+    (only NaN or -inf) gives token 0."""
     assert logits.ndim == 2
+    if min_p > 0.0 or uniform is not None:
+        if vocab_size:
+            logits = logits[:, :vocab_size]
+        if uniform is None:
+            uniform = torch.rand(logits.size(0), device=logits.device)
+        return sample_tokens(
+            logits, uniform, temperature=temperature, top_k=top_k,
+            top_p=top_p, min_p=min_p,
+        ).clamp(min=0)
     assert top_k == 0 or top_p == 0.0, "cannot set both top-k and top-p"
 
     if top_k == 1:  # greedy

@@ -69,6 +69,7 @@ class MegatronServer:
             temperature = float(raw.get("temperature", 1.0))
             top_k = int(raw.get("top_k", 0))
             top_p = float(raw.get("top_p", 0.0))
+            min_p = float(raw.get("min_p", 0.0))
             add_BOS = bool(raw.get("add_BOS", False))
             stop_on_double_eol = bool(raw.get("stop_on_double_eol", False))
             stop_on_eol = bool(raw.get("stop_on_eol", False))
@@ -102,6 +103,7 @@ class MegatronServer:
                         temperature=temperature, add_BOS=add_BOS,
                         stop_on_double_eol=stop_on_double_eol,
                         stop_on_eol=stop_on_eol, random_seed=random_seed,
+                        min_p_sampling=min_p,
                     )
                     resp, segments, output_log_probs, _ = result
                     return JSONResponse({

@@ -22,11 +22,16 @@ import torch
 import torch.nn.functional as F
 
 from .. import parallel as mpu
+from ..ops import QuantKVCache
 from ..ops import functional as ops_f
 from .enums import AttnMaskType, AttnType, LayerType
 from .module import MegatronModule
 from .norms import get_norm
-from .rope import apply_rotary_emb, precompute_freqs
+from .rope import (
+    apply_rotary_emb,
+    precompute_freqs,
+    precompute_rotary_tables,
+)
 
 
 def _args_device():
@@ -278,6 +283,13 @@ class ParallelAttention(MegatronModule):
             world_size=world_size,
         )
 
+        # layouts and scalings beyond the interleaved, whole, linearly scaled
+        # head go through ops.rotary_embedding with tables of their own
+        self.rotary_general = cfg.position_embedding_type == "rotary" and (
+            cfg.rotary_layout != "interleaved" or cfg.rotary_percent != 1.0
+            or cfg.rope_scaling_type != "linear"
+        )
+        self._rotary_tables = {}  # by device
         if cfg.position_embedding_type == "rotary":
             cos, sin = precompute_freqs(
                 self.hidden_size_per_attention_head,
@@ -298,6 +310,71 @@ class ParallelAttention(MegatronModule):
             self.hidden_size_per_attention_head,
             dtype=dtype, device=device,
         )
+
+    def _tables(self, device):
+        """fp32 cos/sin tables of this layer's rotary positions on device."""
+        if not self.rotary_general:
+            return tuple(t.to(device=device, dtype=torch.float32)
+                         for t in (self.rope_cos, self.rope_sin))
+        if device not in self._rotary_tables:
+            cfg = self.cfg
+            dim = int(self.hidden_size_per_attention_head
+                      * cfg.rotary_percent) // 2 * 2
+            self._rotary_tables[device] = precompute_rotary_tables(
+                dim, cfg.max_position_embeddings, theta=cfg.rope_theta,
+                scaling_type=cfg.rope_scaling_type,
+                scaling_factor=cfg.rope_scaling_factor,
+                original_max_position=cfg.rope_original_max_positions
+                or cfg.max_position_embeddings,
+                device=device,
+            )
+        return self._rotary_tables[device]
+
+    def _quant_cache_attend(self, query, key, value, attention_mask,
+                            inference_params):
+        """Generation over keys and values held in 4 bits: positions are
+        rotated, the new tokens appended, and attention runs over the cache. A
+        prompt attends to its own tokens as they were, as training does,
+        unless sinks have to stay visible past its window."""
+        ip = inference_params
+        sq, b, _, hn = query.shape
+        if self.layer_number not in ip.key_value_memory_dict:
+            ip.key_value_memory_dict[self.layer_number] = QuantKVCache(
+                ip.max_sequence_len, b,
+                self.num_attention_heads_kv_per_partition, hn,
+                dtype=key.dtype, device=key.device,
+            )
+        cache = ip.key_value_memory_dict[self.layer_number]
+        window = None
+        if self.use_flash_attn and self.flash_attention.window_size:
+            window = int(self.flash_attention.window_size)
+        sinks = self.cfg.attention_sink_size if window else 0
+        graph = getattr(ip, "use_graph", False) and sq == 1
+        start = ip.graph_pos if graph else ip.sequence_len_offset
+        interleaved = self.cfg.rotary_layout == "interleaved"
+        rotary = self.rope_cos is not None
+        if rotary:
+            cos, sin = self._tables(query.device)
+
+        if not graph and start == 0 and not (sinks and sq > window):
+            if rotary:
+                query, key = ops_f.rotary_embedding(
+                    query, key, cos, sin, interleaved=interleaved
+                )
+            with torch.no_grad():
+                cache.append(key.detach(), value.detach(), 0)
+            return self._attend(query, key, value, attention_mask, ip)
+
+        with torch.no_grad():
+            query, key, value = (t.detach() for t in (query, key, value))
+            if rotary:
+                query = cache.append(key, value, start, query=query, cos=cos,
+                                     sin=sin, interleaved=interleaved)
+            else:
+                cache.append(key, value, start)
+            context = cache.attention(query, start, window_size=window,
+                                      sink_size=sinks)
+        return self.dense(context)
 
     def forward(self, hidden_states, attention_mask, position_ids=None,
                 inference_params=None, encoder_output=None):
@@ -322,6 +399,7 @@ class ParallelAttention(MegatronModule):
             if (
                 mixed.is_cuda
                 and self.rope_cos is not None
+                and not self.rotary_general
                 and inference_params is None
             ):
                 cos = self.rope_cos.to(device=mixed.device,
@@ -357,11 +435,20 @@ class ParallelAttention(MegatronModule):
             key = kv[..., :hn].contiguous()
             value = kv[..., hn:].contiguous()
 
+        if (
+            inference_params is not None
+            and self.cfg.kv_cache_bits == 4
+            and self.attention_type == AttnType.self_attn
+        ):
+            return self._quant_cache_attend(query, key, value,
+                                            attention_mask, inference_params)
+
         # fused decode step: {rope + cache-append}, {attention} — three
         # kernels total (with the dense gemv) instead of the ~20-op eager
         # chain; all positions device-held so the step is graph-capturable
         if (
             self.rope_cos is not None
+            and not self.rotary_general
             and inference_params is not None
             and getattr(inference_params, "use_graph", False)
             and sq == 1
@@ -391,7 +478,21 @@ class ParallelAttention(MegatronModule):
             return self.dense(ctx_row.unsqueeze(0))
 
         # rotary embedding
-        if self.rope_cos is not None:
+        if self.rotary_general:
+            cos, sin = self._tables(query.device)
+            positions = None
+            if inference_params is not None:
+                positions = position_ids
+                if positions is None:
+                    positions = (
+                        inference_params.sequence_len_offset
+                        + torch.arange(sq, device=query.device)
+                    ).unsqueeze(0).expand(b, sq)
+            query, key = ops_f.rotary_embedding(
+                query, key, cos, sin, positions=positions,
+                interleaved=self.cfg.rotary_layout == "interleaved",
+            )
+        elif self.rope_cos is not None:
             # tables stay fp32 regardless of module dtype conversion
             cos = self.rope_cos.to(device=query.device, dtype=torch.float32)
             sin = self.rope_sin.to(device=query.device, dtype=torch.float32)

@@ -1,0 +1,249 @@
+"""Generation with the 4-bit cache, rotary layouts in a model, and combined
+sampling filters: what the serving operators are reached by, on the CPU and on
+the GPU."""
+
+import pytest
+import torch
+
+
+
+@pytest.fixture(params=["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def device(request):
+    if request.param == "cpu" and torch.cuda.is_available():
+        pytest.skip("the framework's device is the GPU")
+    return request.param
+
+
+def make_model(device, seed=5, **change):
+    from megatron_amd import global_state
+    from megatron_amd.config import TrainingConfig, set_config
+    from megatron_amd.models import LlamaModel
+    from megatron_amd.tokenizer.tokenizers import FakeTokenizer
+
+    settings = dict(
+        num_layers=2, hidden_size=256, num_attention_heads=4,
+        num_attention_heads_kv=2, kv_channels=64, seq_length=64,
+        max_position_embeddings=128, micro_batch_size=2, bf16=True,
+        hidden_dropout=0.0, attention_dropout=0.0, use_flash_attn=True,
+        use_cpu_initialization=True, use_hip_graph_decode=False,
+    )
+    cfg = TrainingConfig(**{**settings, **change})
+    cfg.finalize()
+    cfg.pad_vocab_size(100)
+    set_config(cfg)
+    global_state.set_tokenizer(FakeTokenizer(100))
+    torch.manual_seed(seed)
+    model = LlamaModel(cfg, parallel_output=False).to(device).bfloat16()
+    return model.eval(), cfg
+
+
+def steps_of(model, tokens, prompt, total):
+    """Logits of the prompt's last token and of each step behind it."""
+    from megatron_amd.inference.forward_step import ForwardStep
+    from megatron_amd.utils import get_ltor_masks_and_position_ids
+
+    mask, _, ids = get_ltor_masks_and_position_ids(tokens, 0, False, False,
+                                                   False)
+    forward = ForwardStep(model, tokens.shape[0], total)
+    out = []
+    with torch.no_grad():
+        low = 0
+        for high in range(prompt, total):
+            logits = forward(tokens[:, low:high], ids[:, low:high],
+                             mask[..., low:high, :high])
+            out.append(logits[:, -1].float().clone())
+            low = high
+    return out, forward.inference_params
+
+
+def test_four_bit_cache_prompt_as_before_and_steps_near(dist_single, device):
+    """The prompt attends to its tokens as they were; the steps' logits move by
+    what 4 bits lose, which is little of their spread (a value is off by half
+    a thirtieth of its group's range at most, in sums over many)."""
+    torch.manual_seed(1)
+    tokens = torch.randint(1, 99, (2, 40), device=device)
+    plain, _ = make_model(device)
+    want, _ = steps_of(plain, tokens, 20, 40)
+    four, _ = make_model(device, kv_cache_bits=4)
+    four.load_state_dict(plain.state_dict())
+    got, params = steps_of(four, tokens, 20, 40)
+    assert torch.equal(got[0], want[0])
+    for x, y in zip(got, want):
+        assert (x - y).norm() < 0.1 * y.norm()
+    from megatron_amd.ops import QuantKVCache
+
+    assert all(isinstance(c, QuantKVCache)
+               for c in params.key_value_memory_dict.values())
+
+
+def test_four_bit_step_is_attention_over_what_is_held(dist_single, device):
+    """One attention layer's step against the sum over what its cache holds,
+    in 64 bits."""
+    from megatron_amd.inference.forward_step import InferenceParams
+    from megatron_amd.ops.functional import rotate_reference
+
+    model, cfg = make_model(device, kv_cache_bits=4, rotary_layout="half",
+                            rotary_percent=0.5, rope_scaling_type="ntk",
+                            rope_scaling_factor=2.0)
+    attn = model.language_model.encoder.layers[0].self_attention
+    params = InferenceParams(2, 30)
+    torch.manual_seed(2)
+    x = torch.randn(13, 2, 256, device=device).bfloat16()
+    caught = []
+    attn.dense.register_forward_pre_hook(
+        lambda m, args: caught.append(args[0].detach()))
+    with torch.no_grad():
+        attn(x[:12], None, inference_params=params)
+        params.sequence_len_offset = 12
+        attn(x[12:], None, inference_params=params)
+        cache = params.key_value_memory_dict[attn.layer_number]
+        key, value = (t.double().cpu() for t in cache.dequantize(0, 13))
+        mixed, _ = attn.query_key_value(x[12:])
+        q = mixed.view(1, 2, 2, 4 * 64)[..., :128].reshape(1, 2, 4, 64)
+        cos, sin = attn._tables(x.device)
+        q = rotate_reference(q, cos[12].double().expand(1, 2, -1),
+                             sin[12].double().expand(1, 2, -1), False)
+    got = caught[-1].view(2, 4, 64).double().cpu()
+    for i in range(2):
+        for head in range(4):
+            p = torch.softmax(key[:, i, head // 2] @ q[0, i, head].double()
+                              .cpu() / 8.0, 0)
+            want = p @ value[:, i, head // 2]
+            # read back in bf16 (2^-8), fp16 operands (2^-10), rounded (2^-8),
+            # and scores that the keys' rounding moves
+            size = p @ value[:, i, head // 2].abs()
+            moved = 2 * 2.0 ** -8 * (key[:, i, head // 2].abs()
+                                     @ q[0, i, head].double().cpu().abs()
+                                     / 8.0).max()
+            off = (got[i, head] - want).abs()
+            assert (off <= size * (2 * moved + 2.0 ** -6)).all()
+
+
+def test_four_bit_generation_and_beams(dist_single, device):
+    from megatron_amd.inference.generation import (
+        beam_search_and_return_on_first_stage,
+        generate_tokens_probs_and_return_on_first_stage,
+    )
+
+    model, cfg = make_model(device, kv_cache_bits=4)
+    torch.manual_seed(3)
+    tokens = torch.zeros(2, 24, dtype=torch.long, device=device)
+    tokens[:, :8] = torch.randint(1, 99, (2, 8), device=device)
+    lengths = torch.tensor([8, 6], device=device)
+    out, _, _ = generate_tokens_probs_and_return_on_first_stage(
+        model, tokens.clone(), lengths, top_k=20, top_p=0.9, min_p=0.05,
+        use_eod_token_for_early_termination=False)
+    assert out.shape == (2, 24) and (out < 100).all() and (out >= 0).all()
+    one = torch.zeros(1, 16, dtype=torch.long, device=device)
+    one[:, :6] = tokens[:1, :6]
+    best, scores = beam_search_and_return_on_first_stage(
+        model, one, torch.tensor([6], device=device), beam_size=3,
+        stop_token=0, num_return_gen=2, length_penalty=1.0)
+    assert best.shape[0] == 2 and torch.isfinite(scores).all()
+
+
+def test_window_with_sinks_in_generation(dist_single, device):
+    """A prompt beyond its window: the first tokens stay visible only with
+    sinks, and a window that covers everything changes nothing."""
+    torch.manual_seed(4)
+    tokens = torch.randint(1, 99, (2, 40), device=device)
+    runs, weights = {}, None
+    for name, change in (
+        ("whole", dict()), ("wide", dict(sliding_window_size=64)),
+        ("sinks", dict(sliding_window_size=8, attention_sink_size=2)),
+        ("all", dict(sliding_window_size=8, attention_sink_size=40)),
+    ):
+        model, _ = make_model(device, kv_cache_bits=4, **change)
+        if weights is not None:
+            model.load_state_dict(weights)
+        weights = model.state_dict()
+        runs[name], _ = steps_of(model, tokens, 20, 40)
+    assert all(torch.equal(x, y) for x, y in zip(runs["whole"], runs["wide"]))
+    for x, y, z in zip(runs["sinks"], runs["all"], runs["whole"]):
+        assert not torch.equal(x, z)
+        assert (y - z).norm() < 0.1 * z.norm()
+
+
+@pytest.mark.parametrize("train", [False, True])
+def test_half_layout_is_interleaved_with_permuted_rows(dist_single, device, train):
+    """Moving each head's rows of the q and k projections from pairs (2j,
+    2j + 1) to (j, j + h/2) and rotating halves gives the same model. Sums run
+    in another order, so values differ by roundings of bf16."""
+    torch.manual_seed(6)
+    tokens = torch.randint(1, 99, (2, 32), device=device)
+    plain, _ = make_model(device)
+    half, _ = make_model(device, rotary_layout="half")
+    half.load_state_dict(plain.state_dict())
+    order = torch.cat([torch.arange(0, 64, 2), torch.arange(1, 64, 2)])
+    for layer in half.language_model.encoder.layers:
+        weight = layer.self_attention.query_key_value.weight.data
+        rows = weight.view(2, 4, 64, 256)  # per key head: q, q, k, v
+        rows[:, :3] = rows[:, :3][:, :, order.to(device)].clone()
+    ids = torch.arange(32, device=device).expand(2, 32)
+    if not train:
+        with torch.no_grad():
+            a, b = (m(tokens, ids, None).float() for m in (plain, half))
+        assert (a - b).norm() < 2.0 ** -6 * a.norm()
+        got, _ = steps_of(half, tokens, 20, 32)
+        want, _ = steps_of(plain, tokens, 20, 32)
+        for x, y in zip(got, want):
+            assert (x - y).norm() < 2.0 ** -6 * y.norm()
+        return
+    grads = []
+    for m in (plain, half):
+        m(tokens, ids, None, labels=tokens).float().mean().backward()
+        grads.append([p.grad for n, p in m.named_parameters()
+                      if "query_key_value" in n])
+    for a, b in zip(*grads):
+        b = b.view(2, 4, 64, 256).clone()
+        back = torch.empty_like(b)
+        back[:, :3][:, :, order.to(device)] = b[:, :3]
+        back[:, 3] = b[:, 3]
+        a = a.view(2, 4, 64, 256).float()
+        assert (a - back.float()).norm() < 2.0 ** -5 * a.norm()
+
+
+def test_configuration_refuses():
+    from megatron_amd.config import TrainingConfig
+
+    for bad in (dict(kv_cache_bits=8), dict(attention_sink_size=4),
+                dict(attention_sink_size=4, kv_cache_bits=4),
+                dict(rotary_layout="other"), dict(rotary_percent=0.0),
+                dict(rope_scaling_type="other"),
+                dict(rope_scaling_type="yarn"),
+                dict(kv_cache_bits=4, pipeline_model_parallel_size=2,
+                     world_size=2)):
+        with pytest.raises(AssertionError):
+            TrainingConfig(**bad).finalize()
+
+
+def test_sample_with_min_p_and_uniform(device):
+    from megatron_amd.inference.sampling import sample
+
+    logits = torch.tensor([[0.0, 3.0, 2.9, -1.0, 9.0]], device=device)
+    u = torch.tensor([0.99], device=device)
+    assert sample(logits, uniform=u).item() == 4
+    assert sample(logits, uniform=u, vocab_size=4).item() == 2
+    assert sample(logits, uniform=u, vocab_size=4, min_p=0.95).item() == 1
+    assert sample(logits, top_k=2, top_p=0.3, uniform=u,
+                  vocab_size=4).item() == 1
+    drawn = {sample(logits, min_p=0.5, vocab_size=4).item()
+             for _ in range(30)}
+    assert drawn <= {1, 2}
+    void = torch.full((1, 5), float("-inf"), device=device)
+    assert sample(void, uniform=u).item() == 0
+
+
+@pytest.mark.gpu
+def test_four_bit_steps_captured_as_eager(dist_single):
+    """The captured step against the eager one: the same kernels on the same
+    values."""
+    torch.manual_seed(7)
+    tokens = torch.randint(1, 99, (2, 40), device="cuda")
+    model, cfg = make_model("cuda", kv_cache_bits=4,
+                            rotary_layout="half", rotary_percent=0.5)
+    eager, _ = steps_of(model, tokens, 20, 40)
+    cfg.use_hip_graph_decode = True
+    graph, _ = steps_of(model, tokens, 20, 40)
+    for a, b in zip(eager, graph):
+        assert torch.equal(a, b)

@@ -21,6 +21,8 @@ def main():
     p.add_argument("--tokens", type=int, default=128)
     p.add_argument("--batch", type=int, default=1)
     p.add_argument("--prompt", type=int, default=32)
+    p.add_argument("--kv_cache_bits", type=int, default=16,
+                   help="4: keys and values are held in 4 bits")
     args = p.parse_args()
 
     os.environ.setdefault("MASTER_ADDR", "127.0.0.1")
@@ -54,6 +56,7 @@ def main():
         micro_batch_size=args.batch, hidden_dropout=0.0,
         attention_dropout=0.0, bf16=torch.cuda.is_available(),
         use_flash_attn=True, model_name=spec["model_name"],
+        kv_cache_bits=args.kv_cache_bits,
     )
     cfg.finalize()
     cfg.pad_vocab_size(spec["vocab"])
