@@ -540,6 +540,20 @@ __device__ __forceinline__ int wave_total(int v) {
   return __builtin_amdgcn_readlane(wave_scan(v), 63);
 }
 
+// The largest of the wave's numbers, none of them negative.
+__device__ __forceinline__ int wave_most(int v) {
+#define MOST_STEP(CTRL, ROWS) \
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false))
+  MOST_STEP(0x111, 0xf);
+  MOST_STEP(0x112, 0xf);
+  MOST_STEP(0x114, 0xf);
+  MOST_STEP(0x118, 0xf);
+  MOST_STEP(0x142, 0xa);
+  MOST_STEP(0x143, 0xc);
+#undef MOST_STEP
+  return __builtin_amdgcn_readlane(v, 63);
+}
+
 // A workgroup's share of the tokens, settled from where the sequences end:
 // each share has `per` tiles, a multiple of what four waves take at once, and
 // `per` is about the least with which the shares of all sequences are no more
@@ -565,8 +579,7 @@ __device__ __forceinline__ Share share_of(const AttentionArgs& a, int index) {
   int longest = first;
   for (int ib = lane + 64; ib < a.cache.b; ib += 64)
     longest = max(longest, tiles_in(ib));
-  for (int o = 32; o > 0; o >>= 1)
-    longest = max(longest, __shfl_xor(longest, o, WAVE_SIZE));
+  longest = wave_most(longest);
   const int total = total_of([](int n) { return n; });
   int per = max(kLeast / kTile, max((total + a.groups - 1) / a.groups,
                                     (longest + a.chunks - 1) / a.chunks));
@@ -679,7 +692,11 @@ struct TileLds {
 };
 
 // 16 bytes a lane from memory to LDS at `to` + 16 lane. Not known to the
-// compiler as a load: wait_loads() is what orders it.
+// compiler as a load: wait_loads() is what orders it. The second form reads
+// at a uniform address + `offset` of the lane; STEP counts for both sides. (A
+// scalar address that a vector instruction wrote may be read by a load after
+// five cycles, m0 after one: the waits are here, since the compiler does not
+// look into the block.)
 __device__ __forceinline__ void load_to_lds(unsigned to, const void* from) {
   asm volatile(
       "s_mov_b32 m0, %0\n\t"
@@ -690,6 +707,27 @@ __device__ __forceinline__ void load_to_lds(unsigned to, const void* from) {
       : "memory", "m0");
 }
 
+template <int STEP>
+__device__ __forceinline__ void load_to_lds(unsigned to, const void* from,
+                                            unsigned offset) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 4\n\t"
+      "global_load_lds_dwordx4 %1, %2 offset:%3"
+      :
+      : "s"(to), "v"(offset), "s"(from), "n"(STEP)
+      : "memory", "m0");
+}
+
+template <int STEPS>
+__device__ __forceinline__ void load_steps(unsigned to, const void* from,
+                                           unsigned offset) {
+  if constexpr (STEPS >= 1) load_to_lds<0>(to, from, offset);
+  if constexpr (STEPS >= 2) load_to_lds<1024>(to, from, offset);
+  if constexpr (STEPS >= 3) load_to_lds<2048>(to, from, offset);
+  if constexpr (STEPS >= 4) load_to_lds<3072>(to, from, offset);
+}
+
 template <int LEFT>
 __device__ __forceinline__ void wait_loads() {
   asm volatile("s_waitcnt vmcnt(%0)" : : "n"(LEFT) : "memory");
@@ -697,8 +735,8 @@ __device__ __forceinline__ void wait_loads() {
 
 struct HeadMemory {
   const unsigned char *k_codes, *v_codes;
-  const __half *k_meta, *v_meta;
-  long meta_stride;  // from group to group of v_meta
+  const __half *k_meta, *v_meta;  // v_meta: of group 0
+  long meta_stride;               // from group to group of v_meta
 };
 
 template <int H>
@@ -706,18 +744,13 @@ __device__ __forceinline__ void fetch_tile(unsigned to, const HeadMemory& m,
                                            long tile, int lane) {
   using S = HeadShape<H>;
   using L = TileLds<H>;
-  const unsigned char* k = m.k_codes + tile * kTile * (H / 2) + lane * 16;
-  const unsigned char* v =
-      m.v_codes + tile * (kTile / 4) * 128 * S::kQuarters + lane * 16;
+  const unsigned char* k = m.k_codes + tile * kTile * (H / 2);
+  const unsigned char* v = m.v_codes + tile * (kTile / 4) * 128 * S::kQuarters;
   const __half* km = m.k_meta + tile * kTile * S::kGroups * 2;
   const __half* vm = m.v_meta + tile * (kTile / 4) * 8;
   if (H >= 64 || lane < 32)
-#pragma unroll
-    for (int i = 0; i < (kTile * H / 2 + 1023) / 1024; ++i)
-      load_to_lds(to + i * 1024, k + i * 1024);
-#pragma unroll
-  for (int i = 0; i < S::kQuarters; ++i)
-    load_to_lds(to + L::kV + i * 1024, v + i * 1024);
+    load_steps<(kTile * H / 2 + 1023) / 1024>(to, k, lane * 16);
+  load_steps<S::kQuarters>(to + L::kV, v, lane * 16);
   constexpr int kLanes = 8 * S::kGroups;  // 16 bytes each
   const int j = lane - (kLanes < 64 ? kLanes : 0);
   const __half* vm_lane = vm + (j >> 3) * m.meta_stride + (j & 7) * 8;
@@ -813,6 +846,9 @@ void attention_kernel(AttentionArgs a) {
       fetch_tile<H>(mine_at + ahead * L::kBytes, memory,
                     tiles.at(i + 4 * ahead), lane);
 
+  // a negative scale goes to the query, so that the largest product of a row
+  // is its largest score
+  const float sign = a.scale_log2e < 0.f ? -1.f : 1.f;
   for (int mt = wave; mt < MT; mt += 4) {
     const int row = row0 + mt * 16 + r;
     float v[H / 4], peak = 0.f;
@@ -852,7 +888,7 @@ void attention_kernel(AttentionArgs a) {
       h8 y;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        y[i] = (_Float16)__builtin_amdgcn_ldexpf(v[w * 8 + i], -e);
+        y[i] = (_Float16)__builtin_amdgcn_ldexpf(v[w * 8 + i] * sign, -e);
         sum[w * S::kKeyGroups / S::kWords] += (float)y[i];
       }
       q_lds[mt][w][lane] = y;
@@ -867,7 +903,9 @@ void attention_kernel(AttentionArgs a) {
       }
       sum_lds[mt][lane] = y;
     }
-    if (g == 0) c_lds[mt][r] = __builtin_amdgcn_ldexpf(a.scale_log2e, e);
+    if (g == 0)
+      c_lds[mt][r] = fmaxf(
+          __builtin_amdgcn_ldexpf(fabsf(a.scale_log2e), e), 1e-37f);
   }
   __syncthreads();
 
@@ -897,18 +935,18 @@ void attention_kernel(AttentionArgs a) {
     return MT == 1 ? q_reg[w] : q_lds[mt][w][lane];
   };
 
-  for (int slot = 0; i < i_high;
-       i += 4, slot = slot + 1 == kAhead ? 0 : slot + 1) {
+  auto step = [&](auto slot_number) {
+    constexpr int kSlot = decltype(slot_number)::value;
     const int tile = tiles.at(i);
     if (i + 4 * (kAhead - 1) < i_high)
       wait_loads<(kAhead - 1) * L::kLoads>();
     else
       wait_loads<0>();
     TileRegs<H> now;
-    read_tile<H>(now, mine + slot * L::kBytes, lane);
+    read_tile<H>(now, mine + kSlot * L::kBytes, lane);
     asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
     if (i + 4 * kAhead < i_high)
-      fetch_tile<H>(mine_at + slot * L::kBytes, memory,
+      fetch_tile<H>(mine_at + kSlot * L::kBytes, memory,
                     tiles.at(i + 4 * kAhead), lane);
 
     f4 st[MT][2];
@@ -961,20 +999,26 @@ void attention_kernel(AttentionArgs a) {
     for (int mt = 0; mt < MT; ++mt) {
       float sc[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sc[e] = st[mt][e >> 2][e & 3] * c[mt];
+      for (int e = 0; e < 8; ++e) sc[e] = st[mt][e >> 2][e & 3];
       if (partly) {
+        // places in the tile, as 32-bit numbers: all fits where it matters
+        const int last = (int)min(pos[mt] - t_tile, (long)kTile);
+        const int low = a.window > 0
+                            ? (int)max(pos[mt] - a.window - t_tile, -1l)
+                            : -1;
+        const int sink =
+            (int)min(max(a.sinks - t_tile, 0l), (long)kTile);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const long t = t_tile + (e >> 2) * 16 + g * 4 + (e & 3);
-          const bool seen =
-              t <= pos[mt] &&
-              (a.window <= 0 || t > pos[mt] - a.window || t < a.sinks);
+          const int t = (e >> 2) * 16 + g * 4 + (e & 3);
+          const bool seen = (t <= last) & ((t > low) | (t < sink));
           sc[e] = seen ? sc[e] : -INFINITY;
         }
       }
       float peak = sc[0];
 #pragma unroll
       for (int e = 1; e < 8; ++e) peak = fmaxf(peak, sc[e]);
+      peak *= c[mt];
       if (__any(peak > m[mt] + kSlack)) {
         peak = fmaxf(peak, __shfl_xor(peak, 16, WAVE_SIZE));
         peak = fmaxf(peak, __shfl_xor(peak, 32, WAVE_SIZE));
@@ -988,7 +1032,8 @@ void attention_kernel(AttentionArgs a) {
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float w = __builtin_amdgcn_exp2f(sc[e] - m[mt]);
+        const float w =
+            __builtin_amdgcn_exp2f(fmaf(sc[e], c[mt], -m[mt]));
         l[mt] += w;
         p8[mt][e] = (_Float16)w;
         if constexpr (kExact)
@@ -1056,6 +1101,13 @@ void attention_kernel(AttentionArgs a) {
         }
       }
     }
+    };
+  static_assert(kAhead == 2, "two slots take turns");
+  for (; i < i_high; i += 4) {
+    step(std::integral_constant<int, 0>());
+    i += 4;
+    if (i >= i_high) break;
+    step(std::integral_constant<int, 1>());
   }
 
   // join the four waves
