@@ -794,9 +794,11 @@ void attention_kernel(AttentionArgs a) {
   __shared__ h8 q_lds[MT][S::kWords][64];
   __shared__ h8 sum_lds[kExact ? MT : 1][64];  // of q, in two parts
   __shared__ float c_lds[MT][16];
-  __shared__ float ml_lds[4][16][2];
+  __shared__ float ml_lds[MT][4][16][2], row_lds[MT][16][2];
   // the waves' tiles, and once those are used up their outputs
-  constexpr int kRing = 4 * kAhead * L::kBytes, kOut = 4 * 16 * (H + 1) * 4;
+  constexpr int kTogether = MT * H <= 256 ? MT : 1;
+  constexpr int kRing = 4 * kAhead * L::kBytes;
+  constexpr int kOut = kTogether * 4 * 16 * (H + 1) * 4;
   __shared__ __align__(16) unsigned char ring[kRing > kOut ? kRing : kOut];
   float(*o_lds)[16][H + 1] = (float(*)[16][H + 1])ring;
   const int lane = threadIdx.x & 63;
@@ -1110,54 +1112,62 @@ void attention_kernel(AttentionArgs a) {
     step(std::integral_constant<int, 1>());
   }
 
-  // join the four waves
-  __syncthreads();
+  // join the four waves, as many tiles of rows at a time as LDS has room for
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
     float sum = l[mt] + __shfl_xor(l[mt], 16, WAVE_SIZE);
     sum += __shfl_xor(sum, 32, WAVE_SIZE);
-    if (mt) __syncthreads();
     if (g == 0) {
-      ml_lds[wave][r][0] = m[mt];
-      ml_lds[wave][r][1] = sum;
+      ml_lds[mt][wave][r][0] = m[mt];
+      ml_lds[mt][wave][r][1] = sum;
+    }
+  }
+#pragma unroll
+  for (int base = 0; base < MT; base += kTogether) {
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kTogether; ++k) {
+      const int mt = base + k;
+      float top = kUnset, sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) top = fmaxf(top, ml_lds[mt][w][r][0]);
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+        sum += ml_lds[mt][w][r][1] *
+               __builtin_amdgcn_exp2f(ml_lds[mt][w][r][0] - top);
+      if (wave == 0 && g == 0) {
+        row_lds[mt][r][0] = top;
+        row_lds[mt][r][1] = sum;
+      }
+      const float f = __builtin_amdgcn_exp2f(m[mt] - top);
+#pragma unroll
+      for (int j = 0; j < S::kBlocks; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          o_lds[k * 4 + wave][r][(4 * g + e) * S::kBlocks + j] =
+              (o[mt][j][e] + mid[mt][e]) * f;
     }
     __syncthreads();
-    float top = kUnset;
-    for (int w = 0; w < 4; ++w) top = fmaxf(top, ml_lds[w][r][0]);
-    const float f = __builtin_amdgcn_exp2f(m[mt] - top);
+    const int rows = min(a.rows - row0 - base * 16, kTogether * 16);
+    for (int idx = threadIdx.x; idx < rows * H; idx += 256) {
+      const int k = idx / (16 * H), rr = idx / H % 16, d = idx % H;
+      const int row = row0 + base * 16 + idx / H;
+      float y = 0.f;
 #pragma unroll
-    for (int j = 0; j < S::kBlocks; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        o_lds[wave][r][(4 * g + e) * S::kBlocks + j] =
-            (o[mt][j][e] + mid[mt][e]) * f;
-    __syncthreads();
-    for (int idx = threadIdx.x; idx < 16 * H; idx += 256) {
-      const int rr = idx / H, d = idx % H;
-      const int row = row0 + mt * 16 + rr;
-      if (row >= a.rows) break;
-      float y = 0.f, sum = 0.f, high = kUnset;
-      for (int w = 0; w < 4; ++w) {
-        y += o_lds[w][rr][d];
-        high = fmaxf(high, ml_lds[w][rr][0]);
-      }
-      for (int w = 0; w < 4; ++w)
-        sum += ml_lds[w][rr][1] * __builtin_amdgcn_exp2f(ml_lds[w][rr][0] -
-                                                         high);
+      for (int w = 0; w < 4; ++w) y += o_lds[k * 4 + w][rr][d];
+      const float* ml = row_lds[base + k][rr];
       if (a.chunks > 1) {
         const long at = (bh * a.chunks + chunk) * a.rows + row;
         a.part_o[at * H + d] = y;
-        if (d == 0) {
-          a.part_ml[at * 2] = high;
-          a.part_ml[at * 2 + 1] = sum;
-        }
+        if (d < 2) a.part_ml[at * 2 + d] = ml[d];
       } else {
-        const long i = row / a.rep;
-        const int head = kv_head * a.rep + row % a.rep;
-        float z = y / sum;
+        const unsigned i = (unsigned)row / (unsigned)a.rep;
+        const int head = kv_head * a.rep + row - i * a.rep;
+        float z = y / ml[1];
         if (t0 < 0) z = 0.f;
         else if (t0 + i >= a.cache.capacity) z = NAN;
-        T* out = (T*)a.out + ((i * a.cache.b + ib) * a.n + head) * H + d;
+        T* out =
+            (T*)a.out + (((long)i * a.cache.b + ib) * a.n + head) * H + d;
         *out = DTypeTraits<T>::from_float(z);
       }
     }
@@ -1255,8 +1265,8 @@ void launch_attention(AttentionArgs a, hipStream_t stream) {
               "quant_kv: too many queries at once");
   hipLaunchKernelGGL((attention_kernel<T, H, MT>), dim3(grid), dim3(256), 0,
                      stream, a);
-  // few chunks: a wave for a row (2840 rows of 6 chunks: 6.1 us, against 9.6
-  // with four); many: four (256 rows of 24: 5.1 us)
+  // few chunks: a wave for a row (2840 rows of 6 chunks: 4.9 us, against 7.3
+  // with four); many: four (256 rows of 21: 5.1 us)
   if (a.chunks > 1 && a.chunks <= 32)
     hipLaunchKernelGGL((join_kernel<T, H, MT, 1>), dim3((joins + 3) / 4),
                        dim3(256), 0, stream, a);
