@@ -222,7 +222,9 @@ __device__ __forceinline__ void store_scales(const CacheView& cache, long bh,
 // A prompt: a wave takes 512 / h neighbouring positions of one head, aligned
 // to as many, h / 8 lanes and 8 values a lane for each, so that the pairs of
 // tokens that share words of v_codes meet in a wave and all stores are whole
-// words next to each other.
+// words next to each other. 4 x 2047 tokens of 8 heads of 128 take 21 us (41
+// with a row's lanes anywhere, values one by one and pieces of 16 bits); 44 MB
+// are read and written, so that the choice of codes bounds it, not memory.
 template <typename T>
 __global__ __launch_bounds__(256) void append_kernel(CacheView cache,
                                                      AppendSource k,
@@ -281,7 +283,9 @@ __global__ __launch_bounds__(256) void append_kernel(CacheView cache,
 }
 
 // A decode step: a row (token, sequence, head) takes h / 8 lanes with 8 values
-// each. Rows of q come behind those of k and v and are only rotated.
+// each. Rows of q come behind those of k and v and are only rotated. 16 tokens
+// of 32 query and 8 key heads take 6.2 us, one way to memory after another
+// (position, table, codes' 64-bit steps); 10 with values loaded one by one.
 template <typename T>
 __global__ __launch_bounds__(256) void append_rotated_kernel(
     CacheView cache, AppendSource k, AppendSource v, AppendSource q,
@@ -392,7 +396,8 @@ __global__ __launch_bounds__(256) void append_rotated_kernel(
 }
 
 // Reads back with the same lanes as append_kernel; positions outside the cache
-// read as NaN.
+// read as NaN. 4 x 2047 tokens of 8 heads of 128 take 11.4 us, 3.8 TB/s (48
+// with a thread for a value).
 template <typename T>
 __global__ __launch_bounds__(256) void dequantize_kernel(
     CacheView cache, Start start, long length, long tiles,
@@ -471,6 +476,14 @@ __global__ __launch_bounds__(256) void dequantize_kernel(
 // roundings left out is multiplied as well, and the middle of each group,
 // z + 8 s, goes through products of its own in two parts: the output is as far
 // off as the plain form's (2.1e-4) against 4.4e-4 without.
+
+// What bounds it: turning codes into fp16 takes 208 of the 265 instructions
+// that a wave spends on a tile of 5 KB (h = 128). Alone they would take half
+// the time that the tiles take to come from memory; with three waves a SIMD
+// each hides most of the other. Measured (h = 128, bf16): 32 streams of up to
+// 8192 tokens, 8 key heads, 174 MB: 45 to 50 us, 3.5 to 3.9 TB/s; 4 streams of
+// up to 32768, 105 MB: 29 to 33 us. Loads alone take 29 and 22 of those, and a
+// copy reads and writes 4.9 TB/s.
 
 using h2 = __attribute__((ext_vector_type(2))) _Float16;
 using h8 = __attribute__((ext_vector_type(8))) _Float16;

@@ -10,6 +10,11 @@
 // with the pair at (2j, 2j + 1) (interleaved) or (j, j + r) (half); values
 // past 2r are copied. The backward pass is the transpose: the same with -s.
 // A position outside the tables gives NaN; the tables are never read there.
+//
+// Memory bounds it: each value is read and written once, at three operations.
+// 4096 x 4 tokens of 64 heads of 128 values in bf16 take 107 us a direction,
+// 5.0 TB/s, which is what a copy of 2 GB reaches here (4.9); the kernel with a
+// pair a thread took 350.
 
 #include "common.h"
 

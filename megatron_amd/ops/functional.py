@@ -476,8 +476,12 @@ def rotary_embedding(query, key, cos, sin, positions=None, interleaved=True):
         if not positions.is_cuda and positions.numel() and (
                 int(positions.min()) < 0 or int(positions.max()) >= rows):
             raise ValueError("a position lies outside the tables")
-    return RotaryFunction.apply(query, key, cos.contiguous(),
-                                sin.contiguous(), positions, interleaved,
+    cos, sin = cos.contiguous(), sin.contiguous()
+    if not torch.is_grad_enabled() or not (
+            query.requires_grad or (key is not None and key.requires_grad)):
+        return _rotate_pair(query, key, cos, sin, positions, interleaved,
+                            False)
+    return RotaryFunction.apply(query, key, cos, sin, positions, interleaved,
                                 False)
 
 
