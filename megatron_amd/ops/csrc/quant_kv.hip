@@ -736,9 +736,9 @@ template <int STEPS>
 __device__ __forceinline__ void load_steps(unsigned to, const void* from,
                                            unsigned offset) {
   if constexpr (STEPS >= 1) load_to_lds<0>(to, from, offset);
-  if constexpr (STEPS >= 2) load_to_lds<1024>(to, from, offset);
-  if constexpr (STEPS >= 3) load_to_lds<2048>(to, from, offset);
-  if constexpr (STEPS >= 4) load_to_lds<3072>(to, from, offset);
+  if constexpr (STEPS >= 2) load_to_lds<1 * 1024>(to, from, offset);
+  if constexpr (STEPS >= 3) load_to_lds<2 * 1024>(to, from, offset);
+  if constexpr (STEPS >= 4) load_to_lds<3 * 1024>(to, from, offset);
 }
 
 template <int LEFT>
@@ -1510,8 +1510,12 @@ torch::Tensor quant_kv_attention(std::vector<torch::Tensor> buffers,
   const int resident = mt * cache.h <= 128 ? 3 : mt * cache.h <= 256 ? 2 : 1;
   a.groups = (int)std::max<long>(2l * cache.b, 256 * resident / each);
   const long most = (span + kLeast - 1) / kLeast;
+  // and what they leave for the join stays under 128 MB: with that many query
+  // rows the card is full without shares
+  const long room = (1l << 25) / ((long)cache.b * cache.heads * a.rows *
+                                  (cache.h + 2));
   a.chunks = (int)std::max<long>(
-      1, std::min<long>(std::min<long>(most, 256),
+      1, std::min<long>(std::min<long>(most, std::min<long>(room, 256)),
                         4 * (a.groups * each + base - 1) / base));
   TORCH_CHECK(cache.capacity < (1l << 31) && base * a.chunks < (1l << 31) &&
                   a.groups * each < (1l << 31),

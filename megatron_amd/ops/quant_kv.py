@@ -216,6 +216,12 @@ class QuantKVCache:
         at, at_s = self._check_start(start, s)
         if softmax_scale is None:
             softmax_scale = 1.0 / math.sqrt(h)
+        if not math.isfinite(softmax_scale):
+            raise ValueError("softmax_scale must be finite")
+        # beyond the cache both mean all of it
+        if window_size is not None:
+            window_size = min(window_size, self.max_sequence_len)
+        sink_size = min(sink_size, self.max_sequence_len)
         if self.device.type == "cuda":
             return _ext.load(required=True).quant_kv_attention(
                 self.buffers, self.max_sequence_len, query, at, at_s,

@@ -243,6 +243,7 @@ def test_cache_refuses():
         ((q, 8), {}), ((q[:, :, :3], 0), {}), ((q.half(), 0), {}),
         ((q, 0), dict(window_size=0)), ((q, 0), dict(sink_size=1)),
         ((q, 0), dict(window_size=3, sink_size=-1)),
+        ((q, 0), dict(softmax_scale=math.inf)),
         ((q.clone().requires_grad_(), 0), {}),
     ]:
         with pytest.raises(ValueError):

@@ -396,6 +396,108 @@ def test_attention_scale_and_strides():
     assert torch.equal(one, cache.attention(q, 5))
 
 
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 1e-30, 4.0])
+def test_attention_unusual_scales(scale):
+    g = generator(15)
+    cache = filled_cache(g, 300, 2, 2, 64, BF16)
+    q = randn(g, 1, 2, 4, 64, dtype=BF16)
+    got = cache.attention(q.cuda(), torch.tensor([299, 40], device="cuda"),
+                          softmax_scale=scale)
+    want, _ = attention_exact(cache, q, [299, 40], scale, None, 0)
+    bound = attention_exact(cache, q, [299, 40], abs(scale), None, 0)[1]
+    # a bound for |scale| holds its sums with other weights: the largest value
+    # takes their place
+    most = bound.max() + 4.5 * 2.0 ** -8
+    assert ((got.double().cpu() - want).abs() <= most).all()
+
+
+@pytest.mark.parametrize("size", [1e-30, 1e-3, 1e4, 1e30])
+def test_attention_queries_of_any_size(size):
+    """The scale undoes the query's size: the same output, to its roundings
+    (a power of two changes nothing in bf16)."""
+    g = generator(16)
+    cache = filled_cache(g, 100, 1, 1, 128, BF16)
+    q = randn(g, 2, 1, 3, 128, dtype=BF16).cuda()
+    power = 2.0 ** round(math.log2(size))
+    want = cache.attention(q, 98, softmax_scale=0.1)
+    got = cache.attention(q * power, 98, softmax_scale=0.1 / power)
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("b,length", [(65, 700), (150, 300), (3, 9000)])
+def test_attention_many_ragged_sequences(b, length):
+    """Shares of the tokens are settled over all sequences, by waves of 64."""
+    g = generator(b)
+    cache = QuantKVCache(length, b, 2, 64, dtype=BF16, device="cuda")
+    gpu = torch.Generator(device="cuda").manual_seed(b)
+    k, v = (torch.randn(length, b, 2, 64, generator=gpu, device="cuda")
+            .to(BF16) for _ in range(2))
+    cache.append(k, v, 0)
+    q = randn(g, 1, b, 4, 64, dtype=BF16)
+    start = torch.randint(0, length, (b,), generator=g)
+    start[torch.rand(b, generator=g) < 0.2] = -1
+    start[-1] = length - 1
+    out = cache.attention(q.cuda(), start.cuda())
+    for j in range(b):  # one sequence at a time, alone in a cache
+        one = QuantKVCache(length, 1, 2, 64, dtype=BF16, device="cuda")
+        for t, x in zip(one.buffers, cache.buffers):
+            t.copy_(x[j:j + 1])
+        alone = one.attention(q[:, j:j + 1].cuda(), int(start[j]))
+        # shares differ, and so do the sums' roundings in 32 bits: one step
+        # of bf16, or 2^-16 of values up to 5 where terms cancel
+        off = (out[:, j].float() - alone[:, 0].float()).abs()
+        assert (off <= alone[:, 0].float().abs() * 2.0 ** -7
+                + 5 * 2.0 ** -16).all()
+    assert (out[:, start < 0] == 0).all()
+    some = [0, b // 2, b - 1]
+    part = QuantKVCache(length, 3, 2, 64, dtype=BF16)
+    for t, x in zip(part.buffers, cache.buffers):
+        t.copy_(x[some])
+    want, limit = attention_exact(part, q[:, some],
+                                  [int(start[j]) for j in some], 0.125, None,
+                                  0)
+    assert ((out[:, some].double().cpu() - want).abs() <= limit).all()
+
+
+def test_attention_over_a_prompt():
+    """Many query tokens: more rows than shares of the tokens pay for."""
+    g = generator(17)
+    cache = filled_cache(g, 400, 2, 1, 64, FP16)
+    q = randn(g, 300, 2, 3, 64, dtype=FP16)
+    check_attention(cache, q, [100, 17], window=90, sinks=3)
+
+
+def test_attention_window_beyond_everything():
+    g = generator(18)
+    cache = filled_cache(g, 100, 2, 1, 64, BF16)
+    q = randn(g, 1, 2, 3, 64, dtype=BF16).cuda()
+    at = torch.tensor([99, 7], device="cuda")
+    want = cache.attention(q, at)
+    assert torch.equal(want, cache.attention(q, at, window_size=1 << 62,
+                                             sink_size=1 << 62))
+
+
+def test_cache_past_32_bit_offsets():
+    """A head's codes take more than 2^31 bytes."""
+    g = generator(19)
+    length = (1 << 24) + 5000
+    cache = QuantKVCache(length, 1, 1, 256, dtype=BF16, device="cuda")
+    assert cache.k_codes.numel() > 1 << 31
+    x = randn(g, 200, 1, 1, 256, dtype=BF16)
+    small = QuantKVCache(200, 1, 1, 256, dtype=BF16, device="cuda")
+    q = randn(g, 1, 1, 4, 256, dtype=BF16).cuda()
+    small.append(x.cuda(), x.cuda(), 0)
+    for at in (0, length - 200):
+        cache.append(x.cuda(), x.cuda(), at)
+        for a, b in zip(cache.dequantize(at, 200), small.dequantize()):
+            assert torch.equal(a, b)
+        got = cache.attention(q, at + 199, window_size=200)
+        want = small.attention(q, 199)
+        # other shares, other roundings of sums in 32 bits
+        off = (got.float() - want.float()).abs()
+        assert (off <= want.float().abs() * 2.0 ** -7 + 5 * 2.0 ** -16).all()
+
+
 @pytest.mark.parametrize("h", [64, 128])
 def test_attention_nan_stays_where_it_is_seen(h):
     """NaN in a value or a key reaches the queries that see it and no other;
