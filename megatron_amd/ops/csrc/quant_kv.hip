@@ -45,8 +45,10 @@ struct CacheView {
 struct Start {
   const long* at;  // [b] or [1], or null: the scalar counts
   long stride, scalar;
+  // held where a token's number can be added to it or a place taken from it
   __device__ __forceinline__ long of(int ib) const {
-    return at ? at[ib * stride] : scalar;
+    const long t = at ? at[ib * stride] : scalar;
+    return min(max(t, -(1l << 60)), 1l << 60);
   }
 };
 

@@ -278,6 +278,29 @@ def test_append_leaves_other_rows():
         1].isnan().all()
 
 
+@pytest.mark.parametrize("start", [2 ** 63 - 1, 2 ** 63 - 4, 2 ** 62])
+def test_positions_at_the_end_of_64_bits(start):
+    """A position to which a token's number cannot be added is behind the
+    capacity like any other: nothing is written, what is read is NaN."""
+    g = generator(51)
+    cache = QuantKVCache(70, 2, 2, 64, dtype=BF16, device="cuda")
+    fill = randn(g, 70, 2, 2, 64, dtype=BF16).cuda()
+    cache.append(fill, fill, 0)
+    before = [t.clone() for t in cache.buffers]
+    at = torch.tensor([start, -start - 1], device="cuda")
+    more = randn(g, 9, 2, 2, 64, dtype=BF16).cuda()
+    cos, sin = (t.cuda() for t in precompute_rotary_tables(64, 70))
+    cache.append(more, more, at)
+    q = cache.append(more, more, at, query=more, cos=cos, sin=sin)
+    assert q[:, 0].isnan().all() and not q[:, 1].any()
+    for a, b in zip(cache.buffers, before):
+        assert torch.equal(a, b)
+    for x in cache.dequantize(at, 9):
+        assert x.isnan().all()
+    out = cache.attention(more, at)
+    assert out[:, 0].isnan().all() and not out[:, 1].any()
+
+
 def test_append_empty():
     cache = QuantKVCache(4, 2, 1, 64, dtype=BF16, device="cuda")
     none = torch.empty(0, 2, 1, 64, dtype=BF16, device="cuda")
