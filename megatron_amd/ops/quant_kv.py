@@ -119,7 +119,7 @@ class QuantKVCache:
                         f"cache's {self.max_sequence_len}")
             return start, 0
         start = int(start)
-        if start >= 0 and start + s > self.max_sequence_len:
+        if start + s > self.max_sequence_len:
             raise ValueError(f"start {start} + {s} tokens exceed the cache's "
                              f"{self.max_sequence_len}")
         return None, start

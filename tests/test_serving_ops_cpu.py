@@ -208,6 +208,22 @@ def test_cache_nan_reaches_only_who_sees_it():
     assert not out[:4].isnan().any() and out[4:].isnan().all()
 
 
+def test_cache_idle_start_is_bounded_too():
+    """An idle sequence's tokens may reach the capacity, not pass it."""
+    cache = QuantKVCache(8, 1, 1, 32)
+    x = torch.randn(9, 1, 1, 32).to(BF16)
+    cache.append(x, x, -1)
+    assert not cache.attention(x, -1).any()
+    key, _ = cache.dequantize(-1, 9)
+    assert key[0].isnan().all() and not key[1:].any()
+    more = torch.randn(90, 1, 1, 32).to(BF16)
+    for call in (lambda: cache.append(more, more, -1),
+                 lambda: cache.attention(more, -1),
+                 lambda: cache.dequantize(-1, 90)):
+        with pytest.raises(ValueError):
+            call()
+
+
 def test_cache_refuses():
     for bad in (dict(head_dim=96), dict(head_dim=48),
                 dict(dtype=torch.float32), dict(batch_size=0),
