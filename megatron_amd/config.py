@@ -382,9 +382,10 @@ class TrainingConfig:
             )
         assert self.kv_cache_bits in (4, 16), "kv_cache_bits is 4 or 16"
         if self.attention_sink_size:
-            assert self.kv_cache_bits == 4 and self.sliding_window_size, (
-                "attention_sink_size needs kv_cache_bits 4 and a sliding "
-                "window"
+            assert (self.attention_sink_size > 0 and self.kv_cache_bits == 4
+                    and self.sliding_window_size and self.use_flash_attn), (
+                "attention_sink_size needs kv_cache_bits 4, a sliding window "
+                "and use_flash_attn"
             )
         if self.kv_cache_bits == 4:
             assert self.pipeline_model_parallel_size == 1, (

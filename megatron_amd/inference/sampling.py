@@ -30,12 +30,12 @@ def sample(logits, top_k=0, top_p=0.0, temperature=1.0, vocab_size=None,
     """Sample one token per row of logits [b, v]
     (reference sampling.py:45-98).
 
-    With min_p > 0 or uniform (float32 [b] in [0, 1)) the filters combine as in
+    With min_p or uniform (float32 [b] in [0, 1)) the filters combine as in
     ops.sample_tokens, tokens at or past vocab_size are never drawn, and
     uniform defaults to torch.rand. A row that leaves nothing to draw from
     (only NaN or -inf) gives token 0."""
     assert logits.ndim == 2
-    if min_p > 0.0 or uniform is not None:
+    if min_p != 0.0 or uniform is not None:
         if vocab_size:
             logits = logits[:, :vocab_size]
         if uniform is None:

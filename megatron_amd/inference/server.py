@@ -8,6 +8,7 @@ implemented on FastAPI/uvicorn which are available offline. The wire format
 is unchanged.
 """
 
+import math
 import threading
 
 import torch
@@ -77,6 +78,16 @@ class MegatronServer:
             beam_width = raw.get("beam_width", None)
             stop_token = int(raw.get("stop_token", 0))
             length_penalty = float(raw.get("length_penalty", 1.0))
+            # refused here: the other ranks are not waiting for a result yet
+            if not 0.0 <= min_p <= 1.0:
+                return JSONResponse({"message": "min_p must be in 0..1"},
+                                    status_code=400)
+            if min_p and not (0.0 <= temperature < math.inf and top_k >= 0
+                              and 0.0 <= top_p <= 1.0):
+                return JSONResponse(
+                    {"message": "with min_p, temperature and top_k must not "
+                                "be negative and top_p must be in 0..1"},
+                    status_code=400)
 
             with LOCK:
                 try:

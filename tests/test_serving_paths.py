@@ -208,6 +208,10 @@ def test_configuration_refuses():
 
     for bad in (dict(kv_cache_bits=8), dict(attention_sink_size=4),
                 dict(attention_sink_size=4, kv_cache_bits=4),
+                dict(attention_sink_size=-1, kv_cache_bits=4,
+                     sliding_window_size=8),
+                dict(attention_sink_size=4, kv_cache_bits=4,
+                     sliding_window_size=8, use_flash_attn=False),
                 dict(rotary_layout="other"), dict(rotary_percent=0.0),
                 dict(rope_scaling_type="other"),
                 dict(rope_scaling_type="yarn"),
@@ -232,6 +236,36 @@ def test_sample_with_min_p_and_uniform(device):
     assert drawn <= {1, 2}
     void = torch.full((1, 5), float("-inf"), device=device)
     assert sample(void, uniform=u).item() == 0
+
+
+def test_min_p_out_of_range_is_refused():
+    """By sample, and by the server before it calls upon the other ranks."""
+    import asyncio
+    import json
+
+    from megatron_amd.inference.sampling import sample
+    from megatron_amd.inference.server import MegatronServer
+
+    for bad in (-0.5, 1.5, float("nan")):
+        with pytest.raises(ValueError):
+            sample(torch.zeros(1, 4), min_p=bad)
+
+    app = MegatronServer(None)._build_app()
+    endpoint = next(r.endpoint for r in app.routes if r.path == "/api")
+
+    class Request:
+        def __init__(self, **body):
+            self.body = body
+
+        async def json(self):
+            return dict(prompts=["a"], **self.body)
+
+    for bad in (dict(min_p=-0.5), dict(min_p=1.5), dict(min_p=float("nan")),
+                dict(min_p=0.1, temperature=-1.0),
+                dict(min_p=0.1, top_k=-1), dict(min_p=0.1, top_p=2.0)):
+        answer = asyncio.run(endpoint(Request(**bad)))
+        assert answer.status_code == 400
+        assert "min_p" in json.loads(answer.body)["message"]
 
 
 @pytest.mark.gpu
