@@ -56,30 +56,28 @@ __host__ __device__ __forceinline__ int v_quarters(int h) {
   return h >= 64 ? h / 64 : 1;
 }
 
-// 16-bit piece of v_codes with 4 values (2 where h = 32) from value d on
+// 16-bit piece of v_codes with 4 values (2 where h = 32) from value d >= 0 on
+template <int H>
 __device__ __forceinline__ long v_piece(const CacheView& c, long bh, long t,
-                                        int d) {
-  const int per = c.h / 16, q = v_quarters(c.h);
+                                        unsigned d) {
+  constexpr unsigned per = H / 16;
+  constexpr int q = H >= 64 ? H / 64 : 1;
   const int chunk = d / per, quarter = (d % per) / 4;
-  const long block = (bh * (c.room / 4) + t / 4) * 16 + chunk;
+  const long block = (bh * (c.room >> 2) + (t >> 2)) * 16 + chunk;
   return (block * 2 * q + ((t >> 1) & 1) * q + quarter) * 2 + (t & 1);
 }
 
+template <int H>
 __device__ __forceinline__ long v_meta_at(const CacheView& c, long bh, long t,
                                           int group) {
-  return ((bh * (c.h / kGroup) + group) * (c.room / 4) + t / 4) * 8 + (t & 3);
+  return ((bh * (H / kGroup) + group) * (c.room >> 2) + (t >> 2)) * 8 +
+         (t & 3);
 }
 
-// code of x: the nearest whole number of s above z, ties to even. In 32 bits
-// the quotient is off by 16 * 3 * 2^-24 where it is up to 16; nearer to a
-// border than three times that, products in 64 bits decide.
-__device__ __forceinline__ unsigned code_of(float x, float z, float s,
-                                            float inv) {
-  if (!(s > 0.f)) return 0;
-  const float q = (x - z) * inv;
-  const float whole = rintf(q);
-  if (fabsf(fabsf(q - whole) - 0.5f) > 1e-5f)
-    return (unsigned)fminf(fmaxf(whole, 0.f), 15.f);
+// code of x: the nearest whole number of s above z, ties to even, by products
+// in 64 bits; inv is about 1 / s.
+__device__ __forceinline__ float code_between(float x, float z, float s,
+                                              float inv) {
   const double above = (double)x - (double)z;
   float n = floorf((float)above * inv);
   n = fminf(fmaxf(n, 0.f), 15.f);
@@ -92,10 +90,10 @@ __device__ __forceinline__ unsigned code_of(float x, float z, float s,
     n += 1.f;
     rest -= s;
   }
-  const unsigned code = (unsigned)n;
   const double twice = 2.0 * rest;
-  const bool up = twice > (double)s || (twice == (double)s && (code & 1));
-  return up && code < 15 ? code + 1 : code;
+  const bool up =
+      twice > (double)s || (twice == (double)s && ((unsigned)n & 1));
+  return up && n < 15.f ? n + 1.f : n;
 }
 
 // 64 bits to 32, kept as a step of its own: the compiler would join it with a
@@ -150,62 +148,129 @@ __device__ __forceinline__ void load_eight(float (&y)[8], const T* x,
   for (int i = 0; i < 8; ++i) y[i] = DTypeTraits<T>::to_float(v.t[i]);
 }
 
-// Four lanes hold a group's 32 values: codes in the order of the values from
-// the lowest bits up, and its scale and zero point. A NaN counts as 0.
+// Four lanes hold a group's 32 values: codes in the order of the values, and
+// its scale and zero point. A NaN counts as 0.
 struct Held {
-  unsigned code[8];
+  float code[8];
   __half scale, zero;
   bool nan;  // in the group
 };
 
+// v of the lane's neighbour in its group of four, 1 or 2 lanes off
+template <int OFF>
+__device__ __forceinline__ float beside(float v) {
+  constexpr int kOrder = OFF == 1 ? 0xb1 : 0x4e;  // 1 0 3 2 and 2 3 0 1
+  const int i = __float_as_int(v);
+  return __int_as_float(
+      __builtin_amdgcn_update_dpp(i, i, kOrder, 0xf, 0xf, true));
+}
+
+// of three values without a NaN, as they are: fminf would settle signalling
+// ones first
+__device__ __forceinline__ float least(float a, float b, float c) {
+  float y;
+  asm("v_min3_f32 %0, %1, %2, %3" : "=v"(y) : "v"(a), "v"(b), "v"(c));
+  return y;
+}
+
+__device__ __forceinline__ float most(float a, float b, float c) {
+  float y;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(y) : "v"(a), "v"(b), "v"(c));
+  return y;
+}
+
 __device__ __forceinline__ Held hold_eight(const float (&x)[8]) {
   Held y;
-  float v[8], low = INFINITY, high = -INFINITY;
-  int nan = 0;
+  float v[8];
+  bool odd = false;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    nan |= x[i] != x[i];
-    v[i] = x[i] != x[i] ? 0.f : fminf(fmaxf(x[i], -kHeldMax), kHeldMax);
-    low = fminf(low, v[i]);
-    high = fmaxf(high, v[i]);
+    v[i] = x[i];
+    odd |= !(fabsf(x[i]) <= kHeldMax);
   }
+  y.nan = false;
+  if (__any(odd)) {
+    int nan = 0;
 #pragma unroll
-  for (int o = 1; o < 4; o <<= 1) {
-    low = fminf(low, __shfl_xor(low, o, WAVE_SIZE));
-    high = fmaxf(high, __shfl_xor(high, o, WAVE_SIZE));
-    nan |= __shfl_xor(nan, o, WAVE_SIZE);
+    for (int i = 0; i < 8; ++i) {
+      nan |= x[i] != x[i];
+      v[i] = x[i] != x[i] ? 0.f : fminf(fmaxf(x[i], -kHeldMax), kHeldMax);
+    }
+    nan |= __shfl_xor(nan, 1, WAVE_SIZE);
+    nan |= __shfl_xor(nan, 2, WAVE_SIZE);
+    y.nan = nan;
   }
-  y.nan = nan;
+  float low = least(v[0], v[1], v[2]), high = most(v[0], v[1], v[2]);
+  low = least(least(low, v[3], v[4]), v[5], v[6]);
+  high = most(most(high, v[3], v[4]), v[5], v[6]);
+  low = least(low, v[7], v[7]), high = most(high, v[7], v[7]);
+  float other = beside<1>(low);
+  low = least(low, other, other);
+  other = beside<2>(low);
+  low = least(low, other, other);
+  other = beside<1>(high);
+  high = most(high, other, other);
+  other = beside<2>(high);
+  high = most(high, other, other);
   y.zero = __float2half(low);
   const float z = __half2float(y.zero);
   y.scale = __float2half(to_32(((double)high - (double)z) / 15.0));
-  const float s = __half2float(y.scale), inv = 1.f / s;
+  const float s = __half2float(y.scale);
+  const float inv = s > 0.f ? __builtin_amdgcn_rcpf(s) : 0.f;
+  // In 32 bits a quotient is off by 16 * 4 * 2^-24 where it is up to 16 (the
+  // difference, the reciprocal's two and the product's rounding); nearer to a
+  // border than twice that, products in 64 bits decide.
+  constexpr float kNear = 0.5f - 1e-5f;
+  float off[8], far = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) y.code[i] = code_of(v[i], z, s, inv);
+  for (int i = 0; i < 8; ++i) {
+    const float q = (v[i] - z) * inv;
+    const float whole = rintf(q);
+    off[i] = fabsf(q - whole);
+    y.code[i] = __builtin_amdgcn_fmed3f(whole, 0.f, 15.f);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) far = most(far, off[i], off[i + 1]);
+  if (__any(far > kNear)) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (off[i] > kNear && s > 0.f)
+        y.code[i] = code_between(v[i], z, s, inv);
+  }
   return y;
+}
+
+// Four codes in 16 bits, the first one lowest.
+__device__ __forceinline__ unsigned four_codes(float a, float b, float c,
+                                               float d) {
+  return (unsigned)fmaf(fmaf(fmaf(d, 16.f, c), 16.f, b), 16.f, a);
 }
 
 // Codes of a key's word and of a value's, in the cache's order.
 __device__ __forceinline__ unsigned key_word(const Held& y) {
-  unsigned w = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) w |= y.code[i] << ((i >> 1) * 4 + (i & 1) * 16);
-  return w;
+  const float* c = y.code;
+  return four_codes(c[0], c[2], c[4], c[6]) |
+         four_codes(c[1], c[3], c[5], c[7]) << 16;
 }
 
 __device__ __forceinline__ unsigned value_word(const Held& y) {
-  unsigned w = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) w |= y.code[i] << (i * 4);
-  return w;
+  const float* c = y.code;
+  return four_codes(c[0], c[1], c[2], c[3]) |
+         four_codes(c[4], c[5], c[6], c[7]) << 16;
 }
 
-__device__ __forceinline__ int row_any(int v, int lanes) {
-  for (int o = 1; o < lanes; o <<= 1) v |= __shfl_xor(v, o, WAVE_SIZE);
-  return v;
+// v of any of the row's lanes
+template <int LANES>
+__device__ __forceinline__ bool row_any(bool v) {
+  if (!__any(v)) return false;
+  int y = v;
+#pragma unroll
+  for (int o = 1; o < LANES; o <<= 1) y |= __shfl_xor(y, o, WAVE_SIZE);
+  return y;
 }
 
 // The scales and zero points of a row's groups, by the first lane of each.
+template <int H>
 __device__ __forceinline__ void store_scales(const CacheView& cache, long bh,
                                              long pos, int part,
                                              const Held& k, const Held& v,
@@ -214,9 +279,9 @@ __device__ __forceinline__ void store_scales(const CacheView& cache, long bh,
   const __half nan = __ushort_as_half(0x7e00);
   const int group = part / 4;
   const __half2 m = {nan_row ? nan : k.scale, k.zero};
-  ((__half2*)cache.k_meta)[(bh * cache.room + pos) * (cache.h / kGroup) +
-                           group] = m;
-  __half* w = cache.v_meta + v_meta_at(cache, bh, pos, group);
+  ((__half2*)cache.k_meta)[(bh * cache.room + pos) * (H / kGroup) + group] =
+      m;
+  __half* w = cache.v_meta + v_meta_at<H>(cache, bh, pos, group);
   w[0] = v.nan ? nan : v.scale;
   w[4] = v.zero;
 }
@@ -227,25 +292,27 @@ __device__ __forceinline__ void store_scales(const CacheView& cache, long bh,
 // words next to each other. 4 x 2047 tokens of 8 heads of 128 take 21 us (41
 // with a row's lanes anywhere, values one by one and pieces of 16 bits); 44 MB
 // are read and written, so that the choice of codes bounds it, not memory.
-template <typename T>
+template <typename T, int H>
 __global__ __launch_bounds__(256) void append_kernel(CacheView cache,
                                                      AppendSource k,
                                                      AppendSource v, bool wide,
                                                      Start start, long s,
-                                                     long tiles) {
-  const int lanes = cache.h / 8, per = 64 / lanes;
+                                                     unsigned tiles) {
+  constexpr int lanes = H / 8, per = 64 / lanes;
   const int lane = threadIdx.x & 63;
   const int part = lane & (lanes - 1), d0 = part * 8;
-  const long wave =
-      (long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const long bh = wave / tiles;
-  if (bh >= (long)cache.b * cache.heads) return;
-  const int ib = (unsigned)bh / (unsigned)cache.heads;
-  const int head = (int)bh - ib * cache.heads;
+  const unsigned wave =
+      blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const unsigned row = wave / tiles;
+  if (row >= (unsigned)cache.b * cache.heads) return;
+  const long bh = row;
+  const int ib = row / (unsigned)cache.heads;
+  const int head = row - ib * cache.heads;
   const long t = start.of(ib);
   if (t < 0) return;  // idle
   // positions from the begin's tile on
-  const long pos = (t / per + (wave - bh * tiles)) * per + lane / lanes;
+  const long pos = ((t & -per) + (long)(wave - row * tiles) * per) +
+                   lane / lanes;
   const long is = pos - t;
   const bool real = is >= 0 && is < s && pos < cache.capacity;
   float kx[8] = {}, vx[8] = {};
@@ -256,31 +323,31 @@ __global__ __launch_bounds__(256) void append_kernel(CacheView cache,
                (const T*)v.x + is * v.ss + ib * v.bs + head * v.ns + d0, wide);
   }
   const Held hk = hold_eight(kx), hv = hold_eight(vx);
-  const bool nan_row = row_any(hk.nan || hv.nan, lanes);
+  const bool nan_row = row_any<lanes>(hk.nan || hv.nan);
 
   if (real) {
-    ((unsigned*)cache.k_codes)[(bh * cache.room + pos) * (cache.h / 8) +
+    ((unsigned*)cache.k_codes)[(bh * cache.room + pos) * lanes +
                                part] = key_word(hk);
-    store_scales(cache, bh, pos, part, hk, hv, nan_row);
+    store_scales<H>(cache, bh, pos, part, hk, hv, nan_row);
   }
   const unsigned own = value_word(hv);
   const unsigned other = __shfl_xor(own, lanes, WAVE_SIZE);
   const int other_real = __shfl_xor((int)real, lanes, WAVE_SIZE);
   const bool both = real && other_real;
   unsigned short* pieces = (unsigned short*)cache.v_codes;
-  if (cache.h < 64) {  // a piece has two values
+  if (H < 64) {  // a piece has two values
     if (real)
       for (int i = 0; i < 4; ++i)
-        pieces[v_piece(cache, bh, pos, d0 + 2 * i)] = (own >> (8 * i)) & 255;
+        pieces[v_piece<H>(cache, bh, pos, d0 + 2 * i)] = (own >> (8 * i)) & 255;
   } else if (both) {  // one word of two pieces for either token's lane
     const bool odd = pos & 1;
     const unsigned word = odd ? (other >> 16) | (own & 0xffff0000u)
                               : (own & 0xffffu) | (other << 16);
-    const long at = v_piece(cache, bh, pos & ~1l, d0 + (odd ? 4 : 0));
+    const long at = v_piece<H>(cache, bh, pos & ~1l, d0 + (odd ? 4 : 0));
     *(unsigned*)(pieces + at) = word;
   } else if (real) {
-    pieces[v_piece(cache, bh, pos, d0)] = (unsigned short)own;
-    pieces[v_piece(cache, bh, pos, d0 + 4)] = (unsigned short)(own >> 16);
+    pieces[v_piece<H>(cache, bh, pos, d0)] = (unsigned short)own;
+    pieces[v_piece<H>(cache, bh, pos, d0 + 4)] = (unsigned short)(own >> 16);
   }
 }
 
@@ -288,13 +355,13 @@ __global__ __launch_bounds__(256) void append_kernel(CacheView cache,
 // each. Rows of q come behind those of k and v and are only rotated. 16 tokens
 // of 32 query and 8 key heads take 6.2 us, one way to memory after another
 // (position, table, codes' 64-bit steps); 10 with values loaded one by one.
-template <typename T>
+template <typename T, int H>
 __global__ __launch_bounds__(256) void append_rotated_kernel(
     CacheView cache, AppendSource k, AppendSource v, AppendSource q,
     T* __restrict__ q_out, int n, const float* __restrict__ cos_t,
     const float* __restrict__ sin_t, int r, long table_rows, bool interleaved,
     bool wide, Start start, long s) {
-  const int lanes = cache.h / 8;
+  constexpr int lanes = H / 8;
   const unsigned index = blockIdx.x * 256 + threadIdx.x;
   const unsigned row = index / (unsigned)lanes;
   const int part = index & (lanes - 1), d0 = part * 8;
@@ -375,66 +442,67 @@ __global__ __launch_bounds__(256) void append_rotated_kernel(
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       y.t[i] = DTypeTraits<T>::from_float(idle ? 0.f : own[i]);
-    *(uint4*)(q_out + (long)local * cache.h + d0) = y.u;
+    *(uint4*)(q_out + (long)local * H + d0) = y.u;
     return;
   }
   const bool real = !idle && pos < cache.capacity;  // of the whole row
   const Held hk = hold_eight(own), hv = hold_eight(vx);
-  const bool nan_row = row_any(hk.nan || hv.nan, lanes);
+  const bool nan_row = row_any<lanes>(hk.nan || hv.nan);
   if (!real) return;
   const long bh = (long)ib * cache.heads + head;
-  ((unsigned*)cache.k_codes)[(bh * cache.room + pos) * (cache.h / 8) + part] =
+  ((unsigned*)cache.k_codes)[(bh * cache.room + pos) * lanes + part] =
       key_word(hk);
-  store_scales(cache, bh, pos, part, hk, hv, nan_row);
+  store_scales<H>(cache, bh, pos, part, hk, hv, nan_row);
   const unsigned word = value_word(hv);
   unsigned short* pieces = (unsigned short*)cache.v_codes;
-  if (cache.h >= 64) {
-    pieces[v_piece(cache, bh, pos, d0)] = (unsigned short)word;
-    pieces[v_piece(cache, bh, pos, d0 + 4)] = (unsigned short)(word >> 16);
+  if (H >= 64) {
+    pieces[v_piece<H>(cache, bh, pos, d0)] = (unsigned short)word;
+    pieces[v_piece<H>(cache, bh, pos, d0 + 4)] = (unsigned short)(word >> 16);
   } else {  // a piece has two values
     for (int i = 0; i < 4; ++i)
-      pieces[v_piece(cache, bh, pos, d0 + 2 * i)] = (word >> (8 * i)) & 255;
+      pieces[v_piece<H>(cache, bh, pos, d0 + 2 * i)] = (word >> (8 * i)) & 255;
   }
 }
 
 // Reads back with the same lanes as append_kernel; positions outside the cache
 // read as NaN. 4 x 2047 tokens of 8 heads of 128 take 11.4 us, 3.8 TB/s (48
 // with a thread for a value).
-template <typename T>
+template <typename T, int H>
 __global__ __launch_bounds__(256) void dequantize_kernel(
-    CacheView cache, Start start, long length, long tiles,
+    CacheView cache, Start start, long length, unsigned tiles,
     T* __restrict__ k_out, T* __restrict__ v_out) {
-  const int lanes = cache.h / 8, per = 64 / lanes;
+  constexpr int lanes = H / 8, per = 64 / lanes;
   const int lane = threadIdx.x & 63;
   const int part = lane & (lanes - 1), d0 = part * 8;
-  const long wave =
-      (long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const long bh = wave / tiles;
-  if (bh >= (long)cache.b * cache.heads) return;
-  const int ib = (unsigned)bh / (unsigned)cache.heads;
-  const int head = (int)bh - ib * cache.heads;
+  const unsigned wave =
+      blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const unsigned row = wave / tiles;
+  if (row >= (unsigned)cache.b * cache.heads) return;
+  const long bh = row;
+  const int ib = row / (unsigned)cache.heads;
+  const int head = row - ib * cache.heads;
   const long t = start.of(ib);
   // positions from the begin's tile on, rounded down also where it is negative
-  const long tile = (t >= 0 ? t / per : -((per - 1 - t) / per));
-  const long pos = (tile + (wave - bh * tiles)) * per + lane / lanes;
+  const long pos = ((t & -per) + (long)(wave - row * tiles) * per) +
+                   lane / lanes;
   const long is = pos - t;
   if (is < 0 || is >= length) return;
   Eight<T> ky, vy;
   if (pos >= 0 && pos < cache.capacity) {
-    const int groups = cache.h / kGroup, group = part / 4;
+    const int groups = H / kGroup, group = part / 4;
     const long tok = bh * cache.room + pos;
     const unsigned kw = ((const unsigned*)cache.k_codes)[tok * lanes + part];
     const __half2 km = ((const __half2*)cache.k_meta)[tok * groups + group];
     const unsigned short* pieces = (const unsigned short*)cache.v_codes;
     unsigned vw = 0;
-    if (cache.h >= 64) {
-      vw = pieces[v_piece(cache, bh, pos, d0)] |
-           (unsigned)pieces[v_piece(cache, bh, pos, d0 + 4)] << 16;
+    if (H >= 64) {
+      vw = pieces[v_piece<H>(cache, bh, pos, d0)] |
+           (unsigned)pieces[v_piece<H>(cache, bh, pos, d0 + 4)] << 16;
     } else {
       for (int i = 0; i < 4; ++i)
-        vw |= (pieces[v_piece(cache, bh, pos, d0 + 2 * i)] & 255u) << (8 * i);
+        vw |= (pieces[v_piece<H>(cache, bh, pos, d0 + 2 * i)] & 255u) << (8 * i);
     }
-    const __half* vm = cache.v_meta + v_meta_at(cache, bh, pos, group);
+    const __half* vm = cache.v_meta + v_meta_at<H>(cache, bh, pos, group);
     const float ks = __half2float(km.x), kz = __half2float(km.y);
     const float vs = __half2float(vm[0]), vz = __half2float(vm[4]);
 #pragma unroll
@@ -449,7 +517,7 @@ __global__ __launch_bounds__(256) void dequantize_kernel(
     for (int i = 0; i < 8; ++i)
       ky.t[i] = vy.t[i] = DTypeTraits<T>::from_float(NAN);
   }
-  const long at = ((is * cache.b + ib) * cache.heads + head) * cache.h + d0;
+  const long at = ((is * cache.b + ib) * cache.heads + head) * H + d0;
   *(uint4*)(k_out + at) = ky.u;
   *(uint4*)(v_out + at) = vy.u;
 }
@@ -1346,6 +1414,16 @@ AppendSource source_of(const torch::Tensor& x) {
   return AppendSource{x.data_ptr(), x.stride(0), x.stride(1), x.stride(2)};
 }
 
+#define DISPATCH_HEAD(H, FN, T)                                              \
+  do {                                                                       \
+    switch (H) {                                                             \
+      case 32: FN(T, 32); break;                                             \
+      case 64: FN(T, 64); break;                                             \
+      case 128: FN(T, 128); break;                                           \
+      default: FN(T, 256);                                                   \
+    }                                                                        \
+  } while (0)
+
 #define DISPATCH_HALF(TENSOR, FN)                                            \
   do {                                                                       \
     if ((TENSOR).scalar_type() == torch::kBFloat16) {                        \
@@ -1413,25 +1491,29 @@ c10::optional<torch::Tensor> quant_kv_append(
     const long grid =
         (s * cache.b * (cache.heads + (long)n) * (cache.h / 8) + 255) / 256;
     TORCH_CHECK(grid < (1l << 24), "quant_kv: too many tokens at once");
-#define LAUNCH_APPEND(T)                                                     \
-  hipLaunchKernelGGL((append_rotated_kernel<T>), dim3(grid), dim3(256), 0,   \
-                     stream, cache, source_of(key), source_of(value), q,     \
+#define LAUNCH_ROWS(T, H)                                                    \
+  hipLaunchKernelGGL((append_rotated_kernel<T, H>), dim3(grid), dim3(256),   \
+                     0, stream, cache, source_of(key), source_of(value), q,     \
                      (T*)q_out.data_ptr(), n, cos_p, sin_p, r, table_rows,   \
                      interleaved, all_wide, at, s)
+#define LAUNCH_APPEND(T) DISPATCH_HEAD(cache.h, LAUNCH_ROWS, T)
     DISPATCH_HALF(key, LAUNCH_APPEND);
 #undef LAUNCH_APPEND
+#undef LAUNCH_ROWS
     HIP_CHECK(hipGetLastError());
   } else if (s > 0) {
     // the begin may lie anywhere in a wave's tile
     const long per = 512 / cache.h, tiles = (s + per - 2) / per + 1;
     const long grid = ((long)cache.b * cache.heads * tiles + 3) / 4;
-    TORCH_CHECK(grid < (1l << 31), "quant_kv: too many tokens at once");
-#define LAUNCH_APPEND(T)                                                     \
-  hipLaunchKernelGGL((append_kernel<T>), dim3(grid), dim3(256), 0, stream,   \
-                     cache, source_of(key), source_of(value), all_wide, at,  \
-                     s, tiles)
+    TORCH_CHECK(grid < (1l << 30), "quant_kv: too many tokens at once");
+#define LAUNCH_TILES(T, H)                                                   \
+  hipLaunchKernelGGL((append_kernel<T, H>), dim3(grid), dim3(256), 0,        \
+                     stream, cache, source_of(key), source_of(value),        \
+                     all_wide, at, s, (unsigned)tiles)
+#define LAUNCH_APPEND(T) DISPATCH_HEAD(cache.h, LAUNCH_TILES, T)
     DISPATCH_HALF(key, LAUNCH_APPEND);
 #undef LAUNCH_APPEND
+#undef LAUNCH_TILES
     HIP_CHECK(hipGetLastError());
   }
   if (!query.has_value()) return c10::nullopt;
@@ -1452,14 +1534,16 @@ std::vector<torch::Tensor> quant_kv_dequantize(
   if (k.numel() == 0) return {k, v};
   const long per = 512 / cache.h, tiles = (length + per - 2) / per + 1;
   const long grid = ((long)cache.b * cache.heads * tiles + 3) / 4;
-  TORCH_CHECK(grid < (1l << 31), "quant_kv: too many tokens at once");
+  TORCH_CHECK(grid < (1l << 30), "quant_kv: too many tokens at once");
   auto stream = c10::hip::getCurrentHIPStream();
-#define LAUNCH_DEQUANTIZE(T)                                                 \
-  hipLaunchKernelGGL((dequantize_kernel<T>), dim3(grid), dim3(256), 0,       \
-                     stream, cache, at, (long)length, tiles,                 \
+#define LAUNCH_TILES(T, H)                                                   \
+  hipLaunchKernelGGL((dequantize_kernel<T, H>), dim3(grid), dim3(256), 0,    \
+                     stream, cache, at, (long)length, (unsigned)tiles,       \
                      (T*)k.data_ptr(), (T*)v.data_ptr())
+#define LAUNCH_DEQUANTIZE(T) DISPATCH_HEAD(cache.h, LAUNCH_TILES, T)
   DISPATCH_HALF(k, LAUNCH_DEQUANTIZE);
 #undef LAUNCH_DEQUANTIZE
+#undef LAUNCH_TILES
   HIP_CHECK(hipGetLastError());
   return {k, v};
 }
