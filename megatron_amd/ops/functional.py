@@ -392,10 +392,13 @@ def _rotate_pair(query, key, cos, sin, positions, interleaved, inverse):
     ext = _C(cos)
     if ext is not None:
         # the kernel reads strided views with a dense head_dim
-        given = [t if t.stride(-1) == 1 else t.contiguous()
-                 for t in (query, key) if t is not None]
-        out = ext.rotary_apply(given[0], given[1] if len(given) > 1 else None,
-                               cos, sin, positions, interleaved, inverse)
+        if query is not None and query.stride(-1) != 1:
+            query = query.contiguous()
+        if key is not None and key.stride(-1) != 1:
+            key = key.contiguous()
+        first, second = (key, None) if query is None else (query, key)
+        out = ext.rotary_apply(first, second, cos, sin, positions,
+                               interleaved, inverse)
         if query is None:
             return None, out[0]
         return out[0], (out[1] if key is not None else None)
@@ -445,20 +448,23 @@ def rotary_embedding(query, key, cos, sin, positions=None, interleaved=True):
     0..s-1 in every sequence. interleaved: pairs are (2j, 2j + 1), else
     (j, j + r). Positions outside the tables are refused on the CPU and give
     NaN on the GPU. Differentiable in query and key."""
-    if query.dim() != 4:
+    shape = query.shape
+    if len(shape) != 4:
         raise ValueError("query must be [s, b, heads, head_dim]")
-    s, b, _, h = query.shape
+    s, b, _, h = shape
     dtype, device = query.dtype, query.device
     if dtype not in _ROTARY_TYPES:
         raise ValueError(f"rotary_embedding takes fp32, bf16 or fp16, not "
                          f"{dtype}")
-    if key is not None and (
-            key.dim() != 4 or key.shape[0] != s or key.shape[1] != b
-            or key.shape[3] != h or key.dtype != dtype
-            or key.device != device):
-        raise ValueError("key must match the query but for its heads")
-    rows, r = cos.shape if cos.dim() == 2 else (0, 0)
-    if (not 1 <= r <= h // 2 or sin.shape != cos.shape
+    if key is not None:
+        of_key = key.shape
+        if (len(of_key) != 4 or of_key[0] != s or of_key[1] != b
+                or of_key[3] != h or key.dtype != dtype
+                or key.device != device):
+            raise ValueError("key must match the query but for its heads")
+    table = cos.shape
+    rows, r = table if len(table) == 2 else (0, 0)
+    if (not 1 <= r <= h // 2 or sin.shape != table
             or cos.dtype != torch.float32 or sin.dtype != torch.float32
             or cos.device != device or sin.device != device):
         raise ValueError("cos and sin must be float32 [positions, up to "

@@ -89,29 +89,33 @@ class QuantKVCache:
 
     # -- argument checks ----------------------------------------------------
 
-    def _check_rows(self, x, name, heads=None):
-        want = (self.batch_size, self.head_dim)
-        if x.dim() != 4 or (x.shape[1], x.shape[3]) != want:
-            raise ValueError(
-                f"{name} must be [s, {want[0]}, heads, {want[1]}], "
-                f"not {tuple(x.shape)}")
-        if heads is not None and x.shape[2] != heads:
-            raise ValueError(f"{name} must have {heads} heads, "
-                             f"not {x.shape[2]}")
-        if x.dtype != self.dtype or x.device != self.device:
-            raise ValueError(
-                f"{name} must be {self.dtype} on {self.device}, "
-                f"not {x.dtype} on {x.device}")
-        return x if x.stride(-1) == 1 else x.contiguous()
+    # (on the way of each layer's decode step: attributes are read once)
 
-    def _check_start(self, start, s) -> Tuple[Optional[torch.Tensor], int]:
+    def _check_rows(self, x, name, device, heads=None):
+        shape = x.shape
+        if (len(shape) != 4 or shape[1] != self.batch_size
+                or shape[3] != self.head_dim):
+            raise ValueError(
+                f"{name} must be [s, {self.batch_size}, heads, "
+                f"{self.head_dim}], not {tuple(shape)}")
+        if heads is not None and shape[2] != heads:
+            raise ValueError(f"{name} must have {heads} heads, "
+                             f"not {shape[2]}")
+        if x.dtype != self.dtype or x.device != device:
+            raise ValueError(
+                f"{name} must be {self.dtype} on {device}, "
+                f"not {x.dtype} on {x.device}")
+        return x if x.stride(3) == 1 else x.contiguous()
+
+    def _check_start(self, start, s,
+                     device) -> Tuple[Optional[torch.Tensor], int]:
         if isinstance(start, torch.Tensor):
-            if (start.dtype != torch.int64 or start.dim() != 1
-                    or start.shape[0] not in (1, self.batch_size)
-                    or start.device != self.device):
+            shape = start.shape
+            if (len(shape) != 1 or shape[0] not in (1, self.batch_size)
+                    or start.dtype != torch.int64 or start.device != device):
                 raise ValueError(
                     "start must be an int or an int64 tensor with 1 or "
-                    f"{self.batch_size} elements on {self.device}")
+                    f"{self.batch_size} elements on {device}")
             if not start.is_cuda and start.numel():
                 if int(start.max()) + s > self.max_sequence_len:
                     raise ValueError(
@@ -146,22 +150,22 @@ class QuantKVCache:
         rotary_embedding, and the rotated query is returned; an idle
         sequence's is zero. The key is rounded to its type between rotation
         and quantization."""
-        given = [t is not None for t in (query, cos, sin)]
-        if any(given) != all(given):
+        if (query is None) != (cos is None) or (cos is None) != (sin is None):
             raise ValueError("query, cos and sin come together")
         self._check_no_grad(key, value, query)
-        key = self._check_rows(key, "key", self.num_heads_kv)
-        value = self._check_rows(value, "value", self.num_heads_kv)
-        if key.shape != value.shape:
-            raise ValueError("key and value must have the same shape")
+        device = self.device
+        key = self._check_rows(key, "key", device, self.num_heads_kv)
+        value = self._check_rows(value, "value", device, self.num_heads_kv)
         s = key.shape[0]
-        at, at_s = self._check_start(start, s)
+        if value.shape[0] != s:
+            raise ValueError("key and value must have the same shape")
+        at, at_s = self._check_start(start, s, device)
         if query is not None:
-            query = self._check_rows(query, "query")
+            query = self._check_rows(query, "query", device)
             if query.shape[0] != s:
                 raise ValueError("query and key must have as many tokens")
-            _check_tables(cos, sin, self.head_dim, self.device)
-        if self.device.type == "cuda":
+            _check_tables(cos, sin, self.head_dim, device)
+        if device.type == "cuda":
             return _ext.load(required=True).quant_kv_append(
                 self.buffers, self.max_sequence_len, key, value, at, at_s,
                 query, cos, sin, interleaved)
@@ -179,8 +183,9 @@ class QuantKVCache:
             length = self.max_sequence_len - int(start)
         if length < 0:
             raise ValueError("length must not be negative")
-        at, at_s = self._check_start(start, length)
-        if self.device.type == "cuda":
+        device = self.device
+        at, at_s = self._check_start(start, length, device)
+        if device.type == "cuda":
             return tuple(_ext.load(required=True).quant_kv_dequantize(
                 self.buffers, self.max_sequence_len, at, at_s, length,
                 self.dtype == torch.bfloat16))
@@ -202,7 +207,8 @@ class QuantKVCache:
         own among them, and the first `sink_size`. Returns
         [s, b, heads * head_dim]."""
         self._check_no_grad(query)
-        query = self._check_rows(query, "query")
+        device = self.device
+        query = self._check_rows(query, "query", device)
         s, b, n, h = query.shape
         if n < 1 or n % self.num_heads_kv:
             raise ValueError(f"{n} query heads are no multiple of "
@@ -213,7 +219,7 @@ class QuantKVCache:
             raise ValueError("sink_size must not be negative")
         if sink_size and window_size is None:
             raise ValueError("sink_size needs a window_size")
-        at, at_s = self._check_start(start, s)
+        at, at_s = self._check_start(start, s, device)
         if softmax_scale is None:
             softmax_scale = 1.0 / math.sqrt(h)
         if not math.isfinite(softmax_scale):
@@ -222,7 +228,7 @@ class QuantKVCache:
         if window_size is not None:
             window_size = min(window_size, self.max_sequence_len)
         sink_size = min(sink_size, self.max_sequence_len)
-        if self.device.type == "cuda":
+        if device.type == "cuda":
             return _ext.load(required=True).quant_kv_attention(
                 self.buffers, self.max_sequence_len, query, at, at_s,
                 float(softmax_scale), window_size or 0, sink_size)
@@ -327,13 +333,15 @@ class QuantKVCache:
 
 
 def _check_tables(cos, sin, head_dim, device):
-    for t in (cos, sin):
-        if (t.dim() != 2 or t.dtype != torch.float32 or t.device != device
-                or not t.is_contiguous() or t.shape != cos.shape
-                or not 1 <= t.shape[1] <= head_dim // 2):
-            raise ValueError(
-                "cos and sin must be contiguous float32 tables [positions, "
-                f"up to {head_dim // 2}] on {device}")
+    shape = cos.shape
+    if (len(shape) != 2 or not 1 <= shape[1] <= head_dim // 2
+            or sin.shape != shape
+            or cos.dtype != torch.float32 or sin.dtype != torch.float32
+            or cos.device != device or sin.device != device
+            or not cos.is_contiguous() or not sin.is_contiguous()):
+        raise ValueError(
+            "cos and sin must be contiguous float32 tables [positions, "
+            f"up to {head_dim // 2}] on {device}")
 
 
 def _quantize(x):
