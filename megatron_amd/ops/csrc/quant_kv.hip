@@ -56,23 +56,43 @@ __host__ __device__ __forceinline__ int v_quarters(int h) {
   return h >= 64 ? h / 64 : 1;
 }
 
-// 16-bit piece of v_codes with 4 values (2 where h = 32) from value d >= 0 on
+// Places within a head's memory, for a token t counted from a block of four
+// on: the 16-bit piece of v_codes with 4 values (2 where h = 32) from value d
+// on, and a group's scale in v_meta, four before its zero point.
 template <int H>
-__device__ __forceinline__ long v_piece(const CacheView& c, long bh, long t,
-                                        unsigned d) {
-  constexpr unsigned per = H / 16;
-  constexpr int q = H >= 64 ? H / 64 : 1;
-  const int chunk = d / per, quarter = (d % per) / 4;
-  const long block = (bh * (c.room >> 2) + (t >> 2)) * 16 + chunk;
-  return (block * 2 * q + ((t >> 1) & 1) * q + quarter) * 2 + (t & 1);
-}
+struct Pieces {
+  static constexpr unsigned kQuarters = H >= 64 ? H / 64 : 1;
+  static constexpr unsigned kBlock = 64 * kQuarters;  // of four tokens
 
+  static __device__ __forceinline__ unsigned at(unsigned t, unsigned d) {
+    constexpr unsigned per = H / 16;
+    const unsigned chunk = d / per, quarter = (d % per) / 4;
+    return (t >> 2) * kBlock + chunk * 4 * kQuarters +
+           (((t >> 1) & 1) * kQuarters + quarter) * 2 + (t & 1);
+  }
+  static __device__ __forceinline__ long scale_at(const CacheView& c,
+                                                  unsigned t, int group) {
+    return (long)group * (c.room * 2) + (t >> 2) * 8 + (t & 3);
+  }
+};
+
+// A sequence's head from the block of four tokens that holds token t on.
 template <int H>
-__device__ __forceinline__ long v_meta_at(const CacheView& c, long bh, long t,
-                                          int group) {
-  return ((bh * (H / kGroup) + group) * (c.room >> 2) + (t >> 2)) * 8 +
-         (t & 3);
-}
+struct HeadView {
+  unsigned* k_codes;  // these two from token t itself on
+  __half2* k_meta;
+  unsigned short* v_codes;
+  __half* v_meta;
+  unsigned first;  // token t's number in its block
+
+  __device__ __forceinline__ HeadView(const CacheView& c, long bh, long t)
+      : k_codes((unsigned*)c.k_codes + (bh * c.room + t) * (H / 8)),
+        k_meta((__half2*)c.k_meta + (bh * c.room + t) * (H / kGroup)),
+        v_codes((unsigned short*)c.v_codes +
+                (bh * (c.room >> 2) + (t >> 2)) * Pieces<H>::kBlock),
+        v_meta(c.v_meta + bh * (c.room * 2) * (H / kGroup) + (t >> 2) * 8),
+        first(t & 3) {}
+};
 
 // code of x: the nearest whole number of s above z, ties to even, by products
 // in 64 bits; inv is about 1 / s.
@@ -134,16 +154,29 @@ union Eight {
   T t[8];
 };
 
-template <typename T>
-__device__ __forceinline__ void load_eight(float (&y)[8], const T* x,
-                                           bool wide) {
-  Eight<T> v;
-  if (wide) {
+// WIDE: all rows lie at multiples of 16 bytes
+template <bool WIDE, typename T>
+__device__ __forceinline__ void load_eight(Eight<T>& v, const T* x) {
+  if constexpr (WIDE) {
     v.u = *(const uint4*)x;
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v.t[i] = x[i];
   }
+}
+
+// All loads are on their way before any is waited for: left to itself the
+// compiler takes the first one apart before it asks for the next.
+template <typename T>
+__device__ __forceinline__ void hold_all(Eight<T>& a, Eight<T>& b, long& t) {
+  asm volatile(""
+               : "+v"(a.u.x), "+v"(a.u.y), "+v"(a.u.z), "+v"(a.u.w),
+                 "+v"(b.u.x), "+v"(b.u.y), "+v"(b.u.z), "+v"(b.u.w),
+                 "+v"(t));
+}
+
+template <typename T>
+__device__ __forceinline__ void to_floats(float (&y)[8], const Eight<T>& v) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) y[i] = DTypeTraits<T>::to_float(v.t[i]);
 }
@@ -214,7 +247,13 @@ __device__ __forceinline__ Held hold_eight(const float (&x)[8]) {
   high = most(high, other, other);
   y.zero = __float2half(low);
   const float z = __half2float(y.zero);
-  y.scale = __float2half(to_32(((double)high - (double)z) / 15.0));
+  // 32 bits settle the scale where what they may be off by, 3 * 2^-24 of it,
+  // crosses no border of 16 bits
+  const float about = (high - z) * (1.f / 15.f);
+  y.scale = __float2half(about * (1.f - 0x1p-22f));
+  const __half above = __float2half(about * (1.f + 0x1p-22f));
+  if (__any(__half_as_ushort(y.scale) != __half_as_ushort(above)))
+    y.scale = __float2half(to_32(((double)high - (double)z) / 15.0));
   const float s = __half2float(y.scale);
   const float inv = s > 0.f ? __builtin_amdgcn_rcpf(s) : 0.f;
   // In 32 bits a quotient is off by 16 * 4 * 2^-24 where it is up to 16 (the
@@ -226,15 +265,18 @@ __device__ __forceinline__ Held hold_eight(const float (&x)[8]) {
   for (int i = 0; i < 8; ++i) {
     const float q = (v[i] - z) * inv;
     const float whole = rintf(q);
-    off[i] = fabsf(q - whole);
+    off[i] = q - whole;
     y.code[i] = __builtin_amdgcn_fmed3f(whole, 0.f, 15.f);
   }
 #pragma unroll
-  for (int i = 0; i < 8; i += 2) far = most(far, off[i], off[i + 1]);
+  for (int i = 0; i < 8; i += 2)
+    asm("v_max3_f32 %0, %0, |%1|, |%2|"
+        : "+v"(far)
+        : "v"(off[i]), "v"(off[i + 1]));
   if (__any(far > kNear)) {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (off[i] > kNear && s > 0.f)
+      if (fabsf(off[i]) > kNear && s > 0.f)
         y.code[i] = code_between(v[i], z, s, inv);
   }
   return y;
@@ -269,19 +311,21 @@ __device__ __forceinline__ bool row_any(bool v) {
   return y;
 }
 
-// The scales and zero points of a row's groups, by the first lane of each.
+// The scales and zero points of a row's groups, by the first lane of each; the
+// row is `token` tokens from the view's first.
 template <int H>
-__device__ __forceinline__ void store_scales(const CacheView& cache, long bh,
-                                             long pos, int part,
+__device__ __forceinline__ void store_scales(const CacheView& cache,
+                                             const HeadView<H>& to,
+                                             unsigned token, int part,
                                              const Held& k, const Held& v,
                                              bool nan_row) {
   if (part & 3) return;
   const __half nan = __ushort_as_half(0x7e00);
   const int group = part / 4;
   const __half2 m = {nan_row ? nan : k.scale, k.zero};
-  ((__half2*)cache.k_meta)[(bh * cache.room + pos) * (H / kGroup) + group] =
-      m;
-  __half* w = cache.v_meta + v_meta_at<H>(cache, bh, pos, group);
+  to.k_meta[token * (H / kGroup) + group] = m;
+  __half* w =
+      to.v_meta + Pieces<H>::scale_at(cache, to.first + token, group);
   w[0] = v.nan ? nan : v.scale;
   w[4] = v.zero;
 }
@@ -289,13 +333,15 @@ __device__ __forceinline__ void store_scales(const CacheView& cache, long bh,
 // A prompt: a wave takes 512 / h neighbouring positions of one head, aligned
 // to as many, h / 8 lanes and 8 values a lane for each, so that the pairs of
 // tokens that share words of v_codes meet in a wave and all stores are whole
-// words next to each other. 4 x 2047 tokens of 8 heads of 128 take 21 us (41
-// with a row's lanes anywhere, values one by one and pieces of 16 bits); 44 MB
-// are read and written, so that the choice of codes bounds it, not memory.
-template <typename T, int H>
+// words next to each other. 4 x 2047 tokens of 8 heads of 128 take 14 to 15 us
+// (21 with the head size known at run time only, the borders of codes looked
+// at one by one and the value's load behind the key's; 41 with a row's lanes
+// anywhere and pieces of 16 bits). 44 MB are read and written, 9 us at a
+// copy's rate: 355 instructions a wave, mostly the choice of codes, bound it.
+template <typename T, int H, bool WIDE>
 __global__ __launch_bounds__(256) void append_kernel(CacheView cache,
                                                      AppendSource k,
-                                                     AppendSource v, bool wide,
+                                                     AppendSource v,
                                                      Start start, long s,
                                                      unsigned tiles) {
   constexpr int lanes = H / 8, per = 64 / lanes;
@@ -311,56 +357,64 @@ __global__ __launch_bounds__(256) void append_kernel(CacheView cache,
   const long t = start.of(ib);
   if (t < 0) return;  // idle
   // positions from the begin's tile on
-  const long pos = ((t & -per) + (long)(wave - row * tiles) * per) +
-                   lane / lanes;
-  const long is = pos - t;
-  const bool real = is >= 0 && is < s && pos < cache.capacity;
-  float kx[8] = {}, vx[8] = {};
+  const long base = (t & -per) + (long)(wave - row * tiles) * per;
+  if (base >= cache.capacity) return;
+  const int token = lane / lanes;
+  const long is0 = base - t, is = is0 + token;
+  const bool real = is >= 0 && is < s && base + token < cache.capacity;
+  Eight<T> k_raw, v_raw;
+  k_raw.u = v_raw.u = make_uint4(0, 0, 0, 0);
   if (real) {
-    load_eight((float(&)[8])kx,
-               (const T*)k.x + is * k.ss + ib * k.bs + head * k.ns + d0, wide);
-    load_eight((float(&)[8])vx,
-               (const T*)v.x + is * v.ss + ib * v.bs + head * v.ns + d0, wide);
+    const T* kp = (const T*)k.x + is0 * k.ss + ib * k.bs + head * k.ns;
+    const T* vp = (const T*)v.x + is0 * v.ss + ib * v.bs + head * v.ns;
+    load_eight<WIDE>(k_raw, kp + (token * k.ss + d0));
+    load_eight<WIDE>(v_raw, vp + (token * v.ss + d0));
   }
+  long unused = 0;
+  hold_all(k_raw, v_raw, unused);
+  float kx[8], vx[8];
+  to_floats(kx, k_raw);
+  to_floats(vx, v_raw);
   const Held hk = hold_eight(kx), hv = hold_eight(vx);
   const bool nan_row = row_any<lanes>(hk.nan || hv.nan);
 
+  const HeadView<H> to(cache, bh, base);
+  const unsigned place = to.first + token;  // from a block of four on
   if (real) {
-    ((unsigned*)cache.k_codes)[(bh * cache.room + pos) * lanes +
-                               part] = key_word(hk);
-    store_scales<H>(cache, bh, pos, part, hk, hv, nan_row);
+    to.k_codes[lane] = key_word(hk);
+    store_scales<H>(cache, to, token, part, hk, hv, nan_row);
   }
   const unsigned own = value_word(hv);
   const unsigned other = __shfl_xor(own, lanes, WAVE_SIZE);
   const int other_real = __shfl_xor((int)real, lanes, WAVE_SIZE);
   const bool both = real && other_real;
-  unsigned short* pieces = (unsigned short*)cache.v_codes;
   if (H < 64) {  // a piece has two values
     if (real)
       for (int i = 0; i < 4; ++i)
-        pieces[v_piece<H>(cache, bh, pos, d0 + 2 * i)] = (own >> (8 * i)) & 255;
+        to.v_codes[Pieces<H>::at(place, d0 + 2 * i)] = (own >> (8 * i)) & 255;
   } else if (both) {  // one word of two pieces for either token's lane
-    const bool odd = pos & 1;
+    const bool odd = place & 1;
     const unsigned word = odd ? (other >> 16) | (own & 0xffff0000u)
                               : (own & 0xffffu) | (other << 16);
-    const long at = v_piece<H>(cache, bh, pos & ~1l, d0 + (odd ? 4 : 0));
-    *(unsigned*)(pieces + at) = word;
+    *(unsigned*)(to.v_codes +
+                 Pieces<H>::at(place & ~1u, d0 + (odd ? 4 : 0))) = word;
   } else if (real) {
-    pieces[v_piece<H>(cache, bh, pos, d0)] = (unsigned short)own;
-    pieces[v_piece<H>(cache, bh, pos, d0 + 4)] = (unsigned short)(own >> 16);
+    to.v_codes[Pieces<H>::at(place, d0)] = (unsigned short)own;
+    to.v_codes[Pieces<H>::at(place, d0 + 4)] = (unsigned short)(own >> 16);
   }
 }
 
 // A decode step: a row (token, sequence, head) takes h / 8 lanes with 8 values
 // each. Rows of q come behind those of k and v and are only rotated. 16 tokens
-// of 32 query and 8 key heads take 6.2 us, one way to memory after another
-// (position, table, codes' 64-bit steps); 10 with values loaded one by one.
-template <typename T, int H>
+// of 32 query and 8 key heads take 5.0 us, one way to memory after another
+// (position, table) and the rotation's 64-bit steps; 6.2 where loads wait for
+// each other and arguments come by the lane, 10 with values one by one.
+template <typename T, int H, bool WIDE>
 __global__ __launch_bounds__(256) void append_rotated_kernel(
     CacheView cache, AppendSource k, AppendSource v, AppendSource q,
     T* __restrict__ q_out, int n, const float* __restrict__ cos_t,
     const float* __restrict__ sin_t, int r, long table_rows, bool interleaved,
-    bool wide, Start start, long s) {
+    Start start, long s) {
   constexpr int lanes = H / 8;
   const unsigned index = blockIdx.x * 256 + threadIdx.x;
   const unsigned row = index / (unsigned)lanes;
@@ -375,16 +429,20 @@ __global__ __launch_bounds__(256) void append_rotated_kernel(
   const int head = local - token * heads;
   const int is = token / (unsigned)cache.b;
   const int ib = token - is * cache.b;
-  const AppendSource& from = is_q ? q : k;
-  const T* x =
-      (const T*)from.x + is * from.ss + ib * from.bs + head * from.ns;
+  const T* x = (const T*)(is_q ? q.x : k.x) + is * (is_q ? q.ss : k.ss) +
+               ib * (is_q ? q.bs : k.bs) + head * (is_q ? q.ns : k.ns);
   float own[8], vx[8], pair[8], c[8], sn[8];
-  load_eight(own, x + d0, wide);
-  if (!is_q)
-    load_eight(vx,
-               (const T*)v.x + is * v.ss + ib * v.bs + head * v.ns + d0, wide);
-  const long t = start.of(ib);
+  Eight<T> raw, v_raw;
+  // a row of q loads itself again, so that no branch parts the loads
+  const T* vx_row = is_q ? x
+                         : (const T*)v.x + is * v.ss + ib * v.bs + head * v.ns;
+  long t = start.of(ib);
+  load_eight<WIDE>(raw, x + d0);
+  load_eight<WIDE>(v_raw, vx_row + d0);
+  hold_all(raw, v_raw, t);
   const bool idle = t < 0;
+  to_floats(own, raw);
+  to_floats(vx, v_raw);
   const long pos = t + is;
   const bool known = !idle && pos < table_rows;
 
@@ -415,7 +473,8 @@ __global__ __launch_bounds__(256) void append_rotated_kernel(
           own[2 * i + 1] = to_32(y2);
         }
       } else {
-        load_eight(pair, x + (behind ? d0 - r : d0 + r), wide);
+        load_eight<WIDE>(raw, x + (behind ? d0 - r : d0 + r));
+        to_floats(pair, raw);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const double a = (double)own[i] * c[i];
@@ -449,24 +508,24 @@ __global__ __launch_bounds__(256) void append_rotated_kernel(
   const Held hk = hold_eight(own), hv = hold_eight(vx);
   const bool nan_row = row_any<lanes>(hk.nan || hv.nan);
   if (!real) return;
-  const long bh = (long)ib * cache.heads + head;
-  ((unsigned*)cache.k_codes)[(bh * cache.room + pos) * lanes + part] =
-      key_word(hk);
-  store_scales<H>(cache, bh, pos, part, hk, hv, nan_row);
+  const HeadView<H> to(cache, (long)ib * cache.heads + head, pos);
+  to.k_codes[part] = key_word(hk);
+  store_scales<H>(cache, to, 0, part, hk, hv, nan_row);
   const unsigned word = value_word(hv);
-  unsigned short* pieces = (unsigned short*)cache.v_codes;
   if (H >= 64) {
-    pieces[v_piece<H>(cache, bh, pos, d0)] = (unsigned short)word;
-    pieces[v_piece<H>(cache, bh, pos, d0 + 4)] = (unsigned short)(word >> 16);
+    to.v_codes[Pieces<H>::at(to.first, d0)] = (unsigned short)word;
+    to.v_codes[Pieces<H>::at(to.first, d0 + 4)] =
+        (unsigned short)(word >> 16);
   } else {  // a piece has two values
     for (int i = 0; i < 4; ++i)
-      pieces[v_piece<H>(cache, bh, pos, d0 + 2 * i)] = (word >> (8 * i)) & 255;
+      to.v_codes[Pieces<H>::at(to.first, d0 + 2 * i)] =
+          (word >> (8 * i)) & 255;
   }
 }
 
 // Reads back with the same lanes as append_kernel; positions outside the cache
-// read as NaN. 4 x 2047 tokens of 8 heads of 128 take 11.4 us, 3.8 TB/s (48
-// with a thread for a value).
+// read as NaN. 4 x 2047 tokens of 8 heads of 128 take 8.3 us, 5.3 TB/s (11.4
+// with the head size known at run time only, 48 with a thread for a value).
 template <typename T, int H>
 __global__ __launch_bounds__(256) void dequantize_kernel(
     CacheView cache, Start start, long length, unsigned tiles,
@@ -483,26 +542,28 @@ __global__ __launch_bounds__(256) void dequantize_kernel(
   const int head = row - ib * cache.heads;
   const long t = start.of(ib);
   // positions from the begin's tile on, rounded down also where it is negative
-  const long pos = ((t & -per) + (long)(wave - row * tiles) * per) +
-                   lane / lanes;
-  const long is = pos - t;
+  const long base = (t & -per) + (long)(wave - row * tiles) * per;
+  const int token = lane / lanes;
+  const long is0 = base - t, is = is0 + token, pos = base + token;
   if (is < 0 || is >= length) return;
   Eight<T> ky, vy;
   if (pos >= 0 && pos < cache.capacity) {
-    const int groups = H / kGroup, group = part / 4;
-    const long tok = bh * cache.room + pos;
-    const unsigned kw = ((const unsigned*)cache.k_codes)[tok * lanes + part];
-    const __half2 km = ((const __half2*)cache.k_meta)[tok * groups + group];
-    const unsigned short* pieces = (const unsigned short*)cache.v_codes;
+    const HeadView<H> from(cache, bh, base);
+    const unsigned place = from.first + token;
+    const int group = part / 4;
+    const unsigned kw = from.k_codes[lane];
+    const __half2 km = from.k_meta[token * (H / kGroup) + group];
     unsigned vw = 0;
     if (H >= 64) {
-      vw = pieces[v_piece<H>(cache, bh, pos, d0)] |
-           (unsigned)pieces[v_piece<H>(cache, bh, pos, d0 + 4)] << 16;
+      vw = from.v_codes[Pieces<H>::at(place, d0)] |
+           (unsigned)from.v_codes[Pieces<H>::at(place, d0 + 4)] << 16;
     } else {
       for (int i = 0; i < 4; ++i)
-        vw |= (pieces[v_piece<H>(cache, bh, pos, d0 + 2 * i)] & 255u) << (8 * i);
+        vw |= (from.v_codes[Pieces<H>::at(place, d0 + 2 * i)] & 255u)
+              << (8 * i);
     }
-    const __half* vm = cache.v_meta + v_meta_at<H>(cache, bh, pos, group);
+    const __half* vm =
+        from.v_meta + Pieces<H>::scale_at(cache, place, group);
     const float ks = __half2float(km.x), kz = __half2float(km.y);
     const float vs = __half2float(vm[0]), vz = __half2float(vm[4]);
 #pragma unroll
@@ -517,9 +578,10 @@ __global__ __launch_bounds__(256) void dequantize_kernel(
     for (int i = 0; i < 8; ++i)
       ky.t[i] = vy.t[i] = DTypeTraits<T>::from_float(NAN);
   }
-  const long at = ((is * cache.b + ib) * cache.heads + head) * H + d0;
-  *(uint4*)(k_out + at) = ky.u;
-  *(uint4*)(v_out + at) = vy.u;
+  const long at0 = ((is0 * cache.b + ib) * cache.heads + head) * H;
+  const long at = token * ((long)cache.b * cache.heads * H) + d0;
+  *(uint4*)(k_out + at0 + at) = ky.u;
+  *(uint4*)(v_out + at0 + at) = vy.u;
 }
 
 // ---------------------------------------------------------------------------
@@ -1491,14 +1553,20 @@ c10::optional<torch::Tensor> quant_kv_append(
     const long grid =
         (s * cache.b * (cache.heads + (long)n) * (cache.h / 8) + 255) / 256;
     TORCH_CHECK(grid < (1l << 24), "quant_kv: too many tokens at once");
-#define LAUNCH_ROWS(T, H)                                                    \
-  hipLaunchKernelGGL((append_rotated_kernel<T, H>), dim3(grid), dim3(256),   \
-                     0, stream, cache, source_of(key), source_of(value), q,     \
-                     (T*)q_out.data_ptr(), n, cos_p, sin_p, r, table_rows,   \
-                     interleaved, all_wide, at, s)
-#define LAUNCH_APPEND(T) DISPATCH_HEAD(cache.h, LAUNCH_ROWS, T)
+#define LAUNCH_ROWS(T, H, W)                                                 \
+  hipLaunchKernelGGL((append_rotated_kernel<T, H, W>), dim3(grid),           \
+                     dim3(256), 0, stream, cache, source_of(key),            \
+                     source_of(value), q, (T*)q_out.data_ptr(), n, cos_p,    \
+                     sin_p, r, table_rows, interleaved, at, s)
+#define LAUNCH_HEAD(T, H)                                                    \
+  do {                                                                       \
+    if (all_wide) LAUNCH_ROWS(T, H, true);                                   \
+    else LAUNCH_ROWS(T, H, false);                                           \
+  } while (0)
+#define LAUNCH_APPEND(T) DISPATCH_HEAD(cache.h, LAUNCH_HEAD, T)
     DISPATCH_HALF(key, LAUNCH_APPEND);
 #undef LAUNCH_APPEND
+#undef LAUNCH_HEAD
 #undef LAUNCH_ROWS
     HIP_CHECK(hipGetLastError());
   } else if (s > 0) {
@@ -1506,13 +1574,19 @@ c10::optional<torch::Tensor> quant_kv_append(
     const long per = 512 / cache.h, tiles = (s + per - 2) / per + 1;
     const long grid = ((long)cache.b * cache.heads * tiles + 3) / 4;
     TORCH_CHECK(grid < (1l << 30), "quant_kv: too many tokens at once");
-#define LAUNCH_TILES(T, H)                                                   \
-  hipLaunchKernelGGL((append_kernel<T, H>), dim3(grid), dim3(256), 0,        \
-                     stream, cache, source_of(key), source_of(value),        \
-                     all_wide, at, s, (unsigned)tiles)
-#define LAUNCH_APPEND(T) DISPATCH_HEAD(cache.h, LAUNCH_TILES, T)
+#define LAUNCH_TILES(T, H, W)                                                \
+  hipLaunchKernelGGL((append_kernel<T, H, W>), dim3(grid), dim3(256), 0,     \
+                     stream, cache, source_of(key), source_of(value), at, s, \
+                     (unsigned)tiles)
+#define LAUNCH_HEAD(T, H)                                                    \
+  do {                                                                       \
+    if (all_wide) LAUNCH_TILES(T, H, true);                                  \
+    else LAUNCH_TILES(T, H, false);                                          \
+  } while (0)
+#define LAUNCH_APPEND(T) DISPATCH_HEAD(cache.h, LAUNCH_HEAD, T)
     DISPATCH_HALF(key, LAUNCH_APPEND);
 #undef LAUNCH_APPEND
+#undef LAUNCH_HEAD
 #undef LAUNCH_TILES
     HIP_CHECK(hipGetLastError());
   }
