@@ -110,10 +110,15 @@ __global__ __launch_bounds__(256) void rotary_vec_kernel(
     const long p = positions ? positions[ib * p_bs + is * p_ss] : is;
     const bool inside = p >= 0 && p < table_rows;
     const int j = INTERLEAVED ? at / 2 : at;
+    if (inside) {  // once for all, so that the values come together
 #pragma unroll
-    for (int i = 0; i < kTurns; ++i) {
-      c[i] = inside ? cos_t[p * r + j + i] : NAN;
-      s[i] = inside ? sin_t[p * r + j + i] * sign : NAN;
+      for (int i = 0; i < kTurns; ++i) {
+        c[i] = cos_t[p * r + j + i];
+        s[i] = sin_t[p * r + j + i] * sign;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kTurns; ++i) c[i] = s[i] = NAN;
     }
   }
   for (int base = first; base < last; base += kFlight * side) {
