@@ -12,9 +12,9 @@
 // A position outside the tables gives NaN; the tables are never read there.
 //
 // Memory bounds it: each value is read and written once, at three operations.
-// 4096 x 4 tokens of 64 heads of 128 values in bf16 take 107 us a direction,
-// 5.0 TB/s, which is what a copy of 2 GB reaches here (4.9); the kernel with a
-// pair a thread took 350.
+// 4096 x 4 tokens of 64 heads of 128 values in bf16 take 100 us a direction,
+// 5.4 TB/s, a little over what a copy of 2 GB reaches here (4.9); 107 with the
+// loads parted by branches, 350 with a pair a thread.
 
 #include "common.h"
 
@@ -125,16 +125,15 @@ __global__ __launch_bounds__(256) void rotary_vec_kernel(
     Vec x[kFlight], z[kFlight];
 #pragma unroll
     for (int f = 0; f < kFlight; ++f) {
-      const int head = base + f * side;
-      if (head < last) {
-        const bool is_q = head < q.heads;
-        const T* from =
-            is_q ? (const T*)q.x + is * q.ss + ib * q.bs + head * q.ns
-                 : (const T*)k.x + is * k.ss + ib * k.bs +
-                       (head - q.heads) * k.ns;
-        x[f].u = *(const uint4*)(from + at);
-        if (!INTERLEAVED && turns) z[f].u = *(const uint4*)(from + at + r);
-      }
+      // behind the last head that one again: no branch parts the loads
+      const int head = min(base + f * side, last - 1);
+      const bool is_q = head < q.heads;
+      const T* from =
+          is_q ? (const T*)q.x + is * q.ss + ib * q.bs + head * q.ns
+               : (const T*)k.x + is * k.ss + ib * k.bs +
+                     (head - q.heads) * k.ns;
+      x[f].u = *(const uint4*)(from + at);
+      if (!INTERLEAVED) z[f].u = *(const uint4*)(from + (turns ? at + r : at));
     }
 #pragma unroll
     for (int f = 0; f < kFlight; ++f) {
