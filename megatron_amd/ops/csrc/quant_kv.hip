@@ -613,8 +613,8 @@ __global__ __launch_bounds__(256) void dequantize_kernel(
 // that a wave spends on a tile of 5 KB (h = 128). Alone they would take half
 // the time that the tiles take to come from memory; with three waves a SIMD
 // each hides most of the other. Measured (h = 128, bf16): 32 streams of up to
-// 8192 tokens, 8 key heads, 174 MB: 45 to 50 us, 3.5 to 3.9 TB/s; 4 streams of
-// up to 32768, 105 MB: 29 to 33 us. Loads alone take 29 and 22 of those, and a
+// 8192 tokens, 8 key heads, 174 MB: 44 to 49 us, 3.5 to 3.9 TB/s; 4 streams of
+// up to 32768, 105 MB: 27 to 31 us. Loads alone take 29 and 22 of those, and a
 // copy reads and writes 4.9 TB/s.
 
 using h2 = __attribute__((ext_vector_type(2))) _Float16;
@@ -1322,7 +1322,8 @@ void attention_kernel(AttentionArgs a) {
 // Joins the chunks of a row. WAVES waves share a row, each with every
 // WAVES-th chunk, of which lane i holds the i-th one's maximum and sum; each
 // lane has H / 64 values. What a chunk left is read before it is known to be
-// used: one way to memory less.
+// used: one way to memory less. Chunks come eight at a time: one by one, as
+// the compiler leaves a loop with lane reads, 256 rows of 21 took 5.1 us.
 template <typename T, int H, int MT, int WAVES>
 __global__ __launch_bounds__(256) void join_kernel(AttentionArgs a) {
   constexpr int kEach = H >= 64 ? H / 64 : 1;
@@ -1366,12 +1367,27 @@ __global__ __launch_bounds__(256) void join_kernel(AttentionArgs a) {
   float sum = wave_reduce_sum(ml.y * f);
   float y[kEach] = {};
   const float* po = a.part_o + at * H + d;
-#pragma unroll 4
-  for (int c = part; c < used; c += WAVES) {
-    const float fc = __uint_as_float(__builtin_amdgcn_readlane(
-        (int)__float_as_uint(f), c / WAVES));
-    if (d < H)
-      for (int e = 0; e < kEach; ++e) y[e] += po[c * step * H + e] * fc;
+  constexpr int kBatch = 8;  // chunks on their way together
+  for (int base = part; base < used; base += kBatch * WAVES) {
+    float v[kBatch][kEach];
+    // behind the last chunk that one again: no branch parts the loads
+    const int last = base + (used - 1 - base) / WAVES * WAVES;
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int c = min(base + k * WAVES, last);
+      // (with h = 32 half of the lanes have no values: they take the others')
+      for (int e = 0; e < kEach; ++e)
+        v[k][e] = po[c * step * H + e - (d < H ? 0 : H)];
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int c = base + k * WAVES;
+      const float fc = __uint_as_float(__builtin_amdgcn_readlane(
+          (int)__float_as_uint(f), min(c, last) / WAVES));
+      for (int e = 0; e < kEach; ++e)
+        y[e] = c <= last ? fmaf(v[k][e], fc, y[e]) : y[e];
+    }
   }
   if constexpr (WAVES == 1) {
     if (d < H)
@@ -1410,8 +1426,8 @@ void launch_attention(AttentionArgs a, hipStream_t stream) {
               "quant_kv: too many queries at once");
   hipLaunchKernelGGL((attention_kernel<T, H, MT>), dim3(grid), dim3(256), 0,
                      stream, a);
-  // few chunks: a wave for a row (2840 rows of 6 chunks: 4.9 us, against 7.3
-  // with four); many: four (256 rows of 21: 5.1 us)
+  // few chunks: a wave for a row (2840 rows of 6 chunks: 3.8 us; four waves
+  // took half as long again); many: four (256 rows of 21: 4.2 us)
   if (a.chunks > 1 && a.chunks <= 32)
     hipLaunchKernelGGL((join_kernel<T, H, MT, 1>), dim3((joins + 3) / 4),
                        dim3(256), 0, stream, a);
