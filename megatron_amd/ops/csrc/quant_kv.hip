@@ -997,15 +997,14 @@ void attention_kernel(AttentionArgs a) {
   // is its largest score
   const float sign = a.scale_log2e < 0.f ? -1.f : 1.f;
   for (int mt = wave; mt < MT; mt += 4) {
-    const int row = row0 + mt * 16 + r;
+    // behind the last row that one again (it is not put out): no branch parts
+    // the loads
+    const int row = min(row0 + mt * 16 + r, a.rows - 1);
     float v[H / 4], peak = 0.f;
-    const bool real = row < a.rows;
     const unsigned token = (unsigned)row / (unsigned)a.rep;
-    const T* q = (const T*)a.q;
-    if (real)
-      q += (long)token * a.q_ss + ib * a.q_bs +
-           (long)(kv_head * a.rep + row - token * a.rep) * a.q_ns +
-           g * (H / 4);
+    const T* q = (const T*)a.q + (long)token * a.q_ss + ib * a.q_bs +
+                 (long)(kv_head * a.rep + row - token * a.rep) * a.q_ns +
+                 g * (H / 4);
     if (a.q_wide) {
 #pragma unroll
       for (int i = 0; i < H / 4; i += 8) {
@@ -1013,14 +1012,14 @@ void attention_kernel(AttentionArgs a) {
           uint4 u;
           T t[8];
         } y;
-        y.u = real ? *(const uint4*)(q + i) : make_uint4(0, 0, 0, 0);
+        y.u = *(const uint4*)(q + i);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[i + e] = DTypeTraits<T>::to_float(y.t[e]);
       }
     } else {
 #pragma unroll
       for (int i = 0; i < H / 4; ++i)
-        v[i] = real ? DTypeTraits<T>::to_float(q[i]) : 0.f;
+        v[i] = DTypeTraits<T>::to_float(q[i]);
     }
 #pragma unroll
     for (int i = 0; i < H / 4; ++i) peak = fmaxf(peak, fabsf(v[i]));
