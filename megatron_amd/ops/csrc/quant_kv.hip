@@ -613,7 +613,7 @@ __global__ __launch_bounds__(256) void dequantize_kernel(
 // that a wave spends on a tile of 5 KB (h = 128). Alone they would take half
 // the time that the tiles take to come from memory; with three waves a SIMD
 // each hides most of the other. Measured (h = 128, bf16): 32 streams of up to
-// 8192 tokens, 8 key heads, 174 MB: 44 to 49 us, 3.5 to 3.9 TB/s; 4 streams of
+// 8192 tokens, 8 key heads, 174 MB: 41 to 48 us, 3.6 to 4.2 TB/s; 4 streams of
 // up to 32768, 105 MB: 27 to 31 us. Loads alone take 29 and 22 of those, and a
 // copy reads and writes 4.9 TB/s.
 

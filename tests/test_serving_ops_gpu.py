@@ -255,6 +255,49 @@ def test_append_rotated(dtype, interleaved, h, r):
     assert_same_buffers(cpu, gpu)
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_append_many_groups_of_any_scale(dtype):
+    """Scales and codes near a border are decided as exactly as the others:
+    32768 groups whose middles and spans lie anywhere."""
+    g = generator(52)
+    s, b, nkv, h = 1024, 2, 2, 128
+    cpu, gpu = caches(s, b, nkv, h, dtype)
+    rows = [randn(g, s, b, nkv, 4, 32)
+            * 2.0 ** torch.randint(-9, 10, (s, b, nkv, 4, 1), generator=g)
+            + randn(g, s, b, nkv, 4, 1)
+            * 2.0 ** torch.randint(-9, 10, (s, b, nkv, 4, 1), generator=g)
+            for _ in range(2)]
+    k, v = (x.reshape(s, b, nkv, h).to(dtype) for x in rows)
+    cpu.append(k, v, 0)
+    gpu.append(k.cuda(), v.cuda(), 0)
+    assert_same_buffers(cpu, gpu)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("h", [32, 64, 128, 256])
+def test_rows_at_odd_places_as_at_even_ones(dtype, h):
+    """Rows that begin anywhere, one value off among them, give the same
+    bits as rows at multiples of 16 bytes."""
+    g = generator(53 + h)
+    s, b, n, nkv, length = 5, 2, 6, 2, 50
+    packed = randn(g, s, b, n + 2 * nkv, h + 3, dtype=dtype).cuda()
+    odd = packed[..., 1:h + 1].split([n, nkv, nkv], dim=2)
+    even = [x.contiguous() for x in odd]
+    cos, sin = (t.cuda() for t in precompute_rotary_tables(h, length))
+    at = torch.tensor([3, 40], device="cuda")
+    got = []
+    for q, k, v in (odd, even):
+        cache = QuantKVCache(length, b, nkv, h, dtype=dtype, device="cuda")
+        cache.append(k, v, at - 3)
+        rows = [x.clone() for x in cache.buffers]
+        turned = cache.append(k, v, at, query=q, cos=cos, sin=sin)
+        got.append(rows + cache.buffers
+                   + [turned, cache.attention(q, at),
+                      cache.attention(q[:1], at)])
+    for x, y in zip(*got):
+        assert torch.equal(x, y)
+
+
 def test_append_leaves_other_rows():
     """Idle sequences and rows behind the capacity stay as they were."""
     g = generator(5)
