@@ -311,6 +311,12 @@ class ParallelAttention(MegatronModule):
             dtype=dtype, device=device,
         )
 
+    def _window(self):
+        """Tokens that a decode step sees, its own among them; 0: all."""
+        if self.use_flash_attn and self.flash_attention.window_size:
+            return int(self.flash_attention.window_size)
+        return 0
+
     def _tables(self, device):
         """fp32 cos/sin tables of this layer's rotary positions on device."""
         if not self.rotary_general:
@@ -345,9 +351,7 @@ class ParallelAttention(MegatronModule):
                 dtype=key.dtype, device=key.device,
             )
         cache = ip.key_value_memory_dict[self.layer_number]
-        window = None
-        if self.use_flash_attn and self.flash_attention.window_size:
-            window = int(self.flash_attention.window_size)
+        window = self._window() or None
         sinks = self.cfg.attention_sink_size if window else 0
         graph = getattr(ip, "use_graph", False) and sq == 1
         start = ip.graph_pos if graph else ip.sequence_len_offset
@@ -470,11 +474,9 @@ class ParallelAttention(MegatronModule):
                 query[0], key[0], value[0], cos, sin, ip.graph_pos,
                 k_cache, v_cache,
             )
-            win = -1
-            if self.use_flash_attn and self.flash_attention.window_size:
-                win = int(self.flash_attention.window_size)
             ctx_row = _m.decode_attn(q_rot, k_cache, v_cache, ip.graph_pos,
-                                     1.0 / math.sqrt(hn), win)
+                                     1.0 / math.sqrt(hn),
+                                     self._window() or -1)
             return self.dense(ctx_row.unsqueeze(0))
 
         # rotary embedding
@@ -566,7 +568,7 @@ class ParallelAttention(MegatronModule):
 
             ctx_row = _oext.load(required=True).decode_attn(
                 query[0].contiguous(), k_cache, v_cache, ip.graph_pos,
-                1.0 / math.sqrt(hn),
+                1.0 / math.sqrt(hn), self._window() or -1,
             )
             output, bias = self.dense(ctx_row.unsqueeze(0))
             return output, bias
@@ -585,9 +587,9 @@ class ParallelAttention(MegatronModule):
         scale = 1.0 / math.sqrt(hn)
         scores = torch.bmm(q.float(), k.float().transpose(1, 2)) * scale
         invalid = ip.graph_arange > ip.graph_pos  # [L] device-side length
-        if self.use_flash_attn and self.flash_attention.window_size:
+        w = self._window()
+        if w:
             # sliding window (HF/Mistral: keep w keys incl. current)
-            w = int(self.flash_attention.window_size)
             invalid = invalid | (ip.graph_arange < ip.graph_pos - w + 1)
         scores = scores.masked_fill(invalid.view(1, 1, L), float("-inf"))
         probs = torch.softmax(scores, dim=-1).to(v.dtype)

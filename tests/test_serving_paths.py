@@ -281,3 +281,38 @@ def test_four_bit_steps_captured_as_eager(dist_single):
     graph, _ = steps_of(model, tokens, 20, 40)
     for a, b in zip(eager, graph):
         assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rotary", [
+    dict(),  # the layout whose step is fused with the rotation
+    dict(rotary_layout="half"),
+    dict(rotary_layout="half", rotary_percent=0.25),
+    dict(rope_scaling_type="ntk", rope_scaling_factor=2.0),
+    dict(rope_scaling_type="yarn", rope_scaling_factor=4.0,
+         rope_original_max_positions=32),
+], ids=["plain", "half", "part", "ntk", "yarn"])
+@pytest.mark.parametrize("kv_channels", [64, 128])
+def test_captured_steps_keep_the_window(dist_single, rotary, kv_channels):
+    """Captured steps past the window against the whole sequence at once, as
+    in training, and far from what a model without the window gives. Both sides
+    round to bf16 in another order: 2^-8 at each of two layers' few steps."""
+    torch.manual_seed(8)
+    tokens = torch.randint(1, 99, (2, 48), device="cuda")
+    change = dict(sliding_window_size=6, use_hip_graph_decode=True,
+                  kv_channels=kv_channels, init_method_std=0.1, **rotary)
+    model, _ = make_model("cuda", **change)
+    got, params = steps_of(model, tokens, 20, 48)
+    assert params.use_graph
+    ids = torch.arange(48, device="cuda").expand(2, 48)
+    with torch.no_grad():
+        want = model(tokens, ids, None).float()
+    wide, _ = make_model("cuda", **{**change, "sliding_window_size": None})
+    wide.load_state_dict(model.state_dict())
+    with torch.no_grad():
+        whole = wide(tokens, ids, None).float()
+    for i, x in enumerate(got):
+        at = 19 + i
+        size = want[:, at].norm()
+        assert (whole[:, at] - want[:, at]).norm() > 2.0 ** -3 * size
+        assert (x - want[:, at]).norm() < 2.0 ** -5 * size, at
