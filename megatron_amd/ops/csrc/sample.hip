@@ -96,6 +96,8 @@ struct Lds {
   u64 wave[2][kWaves];
   u64 answer[4];
   float extreme[2][kWaves];
+  u64 found_above;
+  float found;
   unsigned listed, low, high;
 };
 
@@ -427,6 +429,8 @@ __device__ Cut find_cut(Lds& lds, const Row<T>& row, const Weights& weights,
     low = key_value(lds.low);
     high = key_value(lds.high);
     const int listed = (int)lds.listed;
+    // the ranking's answer has a word of its own: a wave that comes late still
+    // reads the bin's extremes above, so that all waves take the same way
     if (low < high && listed <= kList) {
       const int at = tid >> 2;  // four threads rank a token
       if (at < listed) {
@@ -444,13 +448,13 @@ __device__ Cut find_cut(Lds& lds, const Row<T>& row, const Weights& weights,
         larger += above;
         if (MASS ? larger <= limit && larger + equal > limit
                  : larger < limit && larger + equal >= limit) {
-          lds.low = order_key(own_v);
-          lds.answer[3] = larger;
+          lds.found = own_v;
+          lds.found_above = larger;
         }
       }
       __syncthreads();
-      low = high = key_value(lds.low);
-      above = lds.answer[3];
+      low = high = lds.found;
+      above = lds.found_above;
     }
     __syncthreads();
   }

@@ -900,3 +900,29 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(x, want[i]) for x in got[i])
+
+
+@pytest.mark.parametrize("by", ["top_k", "top_p"])
+def test_sample_cuts_at_any_place_of_a_bin(by):
+    """Filters that keep more tokens than are listed, with the cut at each of a
+    bin's few logits in turn, its largest among them. All tokens weigh the same
+    (the temperature is 1e30), so that the last kept index is the one drawn and
+    tells the number of kept tokens; each row draws the same in every run."""
+    g = generator(40)
+    rows, vocab = 700, 4096
+    place = torch.stack([torch.randperm(vocab, generator=g)
+                         for _ in range(rows)])
+    logits = torch.empty(rows, vocab).scatter_(
+        1, place, torch.linspace(9.0, -9.0, vocab).expand(rows, vocab))
+    kept = 257 + torch.arange(rows)
+    if by == "top_k":
+        setting = kept
+    else:  # before the last kept token lie kept - 1
+        setting = (kept - 0.5).float() / vocab
+    uniform = torch.full((rows,), 1.0 - 2.0 ** -24)
+    among = torch.arange(vocab)[None] < kept[:, None]
+    want = place.masked_fill(~among, -1).amax(1)
+    for _ in range(5):
+        got = sample_tokens(logits.cuda(), uniform.cuda(), temperature=1e30,
+                            **{by: setting.cuda()})
+        assert torch.equal(got.cpu(), want)
