@@ -602,9 +602,16 @@ __global__ __launch_bounds__(256) void dequantize_kernel(
 // Codes become fp16 by or-ing them into 1024 + code, which is exact, and one
 // rounded multiply-add by the group's scale and zero point. Query rows are
 // brought to a maximum in [1, 2) by a power of two first, so that bf16 values
-// are exact in fp16 too. Sums and statistics are held in 32 bits. The operands
-// are rounded to fp16, a relative 2^-11 at most, under the 2^-8 of a bf16
-// output. That of an fp16 output is 2^-11 too, so there (EXACT) what the
+// are exact in fp16 too. Sums and statistics are held in 32 bits.
+//
+// For a bf16 output held keys, held values and weights are operands in fp16,
+// each rounded by a relative 2^-11 at most, under the output's own 2^-8: three
+// bits more than keys and values have in a cache of the model's type. What
+// 32-bit operands would take is in the fp16 path: three products for one. A
+// weight under 2^-21 of the wave's largest is held to 2^-32 of that one
+// (kLift), so that n tokens are off by n 2^-32 of the largest value at most.
+//
+// The rounding of an fp16 output is 2^-11 too, so there (EXACT) what the
 // roundings left out is multiplied as well, and the middle of each group,
 // z + 8 s, goes through products of its own in two parts: the output is as far
 // off as the plain form's (2.1e-4) against 4.4e-4 without.
@@ -624,7 +631,10 @@ using f4 = __attribute__((ext_vector_type(4))) float;
 constexpr int kTile = 32;       // tokens of a wave's step
 constexpr int kLeast = 128;     // tokens of a workgroup at least
 constexpr float kUnset = -3e38f;  // maximum before the first score
-constexpr float kSlack = 8.f;   // weights reach 2^8 before the maximum moves
+// Weights are 2^(score - m) with m = the running maximum - kLift, and m stays
+// until a score passes it by kLift + kSlack: they reach 2^15, just under fp16's
+// largest, so that small ones keep what fp16 has under the largest.
+constexpr float kLift = 7.f, kSlack = 8.f;
 
 struct AttentionArgs {
   CacheView cache;
@@ -1165,10 +1175,10 @@ void attention_kernel(AttentionArgs a) {
 #pragma unroll
       for (int e = 1; e < 8; ++e) peak = fmaxf(peak, sc[e]);
       peak *= c[mt];
-      if (__any(peak > m[mt] + kSlack)) {
+      if (__any(peak > m[mt] + (kLift + kSlack))) {
         peak = fmaxf(peak, __shfl_xor(peak, 16, WAVE_SIZE));
         peak = fmaxf(peak, __shfl_xor(peak, 32, WAVE_SIZE));
-        const float up = fmaxf(m[mt], peak);
+        const float up = fmaxf(m[mt], peak - kLift);
         const float alpha = __builtin_amdgcn_exp2f(m[mt] - up);
         m[mt] = up;
         l[mt] *= alpha;

@@ -926,3 +926,28 @@ def test_sample_cuts_at_any_place_of_a_bin(by):
         got = sample_tokens(logits.cuda(), uniform.cuda(), temperature=1e30,
                             **{by: setting.cuda()})
         assert torch.equal(got.cpu(), want)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("gap", [16, 22, 26, 30, 33])
+def test_attention_small_weights_count(dtype, gap):
+    """A token whose value is 0 weighs 2^gap times each other one, whose value
+    is 1, all read by one wave: the output is what the others weigh, also where
+    a weight is under fp16's least against the largest. A weight is held to
+    2^-32 of the wave's largest."""
+    h, tokens = 64, 32
+    cache = QuantKVCache(tokens, 1, 1, h, dtype=dtype, device="cuda")
+    key = torch.zeros(tokens, 1, 1, h, dtype=dtype, device="cuda")
+    value = torch.ones_like(key)
+    key[5], value[5] = 1.0, 0.0
+    cache.append(key, value, 0)
+    q = torch.ones(1, 1, 1, h, dtype=dtype, device="cuda")
+    got = cache.attention(q, tokens - 1,
+                          softmax_scale=gap * math.log(2.0) / h).double()
+    least = 31 * 2.0 ** -gap
+    want = least / (1 + least)
+    # the output's rounding (fp16: its subnormals' too), and each weight's:
+    # 2^-11 of itself (2^-22 in two parts), a 32-bit score's of up to 33
+    limit = (want * (half_step(dtype) + 2.0 ** -11 + 33 * 2.0 ** -22)
+             + 31 * 2.0 ** -32 + (2.0 ** -25 if dtype == FP16 else 0.0))
+    assert ((got - want).abs() <= limit).all(), (got.flatten()[0], want)
