@@ -271,3 +271,109 @@ def test_merge_meta_llama(tmp_path):
                        full["layers.0.attention.wk.weight"])
     assert torch.equal(hf["model.layers.0.self_attn.v_proj.weight"],
                        full["layers.0.attention.wv.weight"])
+
+
+ROTARY = [
+    dict(rotary_layout="half"),
+    dict(rotary_layout="half", rope_theta=500000.0),
+    dict(rope_scaling_factor=2.0),
+    dict(rope_scaling_type="ntk", rope_scaling_factor=4.0),
+    dict(rotary_layout="half", rope_scaling_type="yarn",
+         rope_scaling_factor=4.0, rope_original_max_positions=16),
+]
+
+
+def _checkpoint_of(path, **rotary):
+    """A tiny model with these rotary settings, saved as the exporter reads
+    it; the model."""
+    from megatron_amd.checkpointing import _config_to_namespace
+    from megatron_amd.models import LlamaModel
+
+    cfg = TrainingConfig(
+        num_layers=2, hidden_size=64, ffn_hidden_size=176,
+        num_attention_heads=4, num_attention_heads_kv=2, seq_length=32,
+        max_position_embeddings=64, micro_batch_size=1, hidden_dropout=0.0,
+        attention_dropout=0.0, use_cpu_initialization=True,
+        use_flash_attn=False, init_method_std=0.2, layernorm_epsilon=1e-5,
+        **rotary)
+    cfg.finalize()
+    cfg.padded_vocab_size = 128
+    set_config(cfg)
+    torch.manual_seed(13)
+    model = LlamaModel(cfg, parallel_output=False).eval()
+    place = path / "release" / "mp_rank_00"
+    place.mkdir(parents=True)
+    torch.save({"args": _config_to_namespace(cfg),
+                "model": {"language_model":
+                          model.language_model.state_dict()}},
+               place / "model_optim_rng.pt")
+    (path / "latest_checkpointed_iteration.txt").write_text("release")
+    return model
+
+
+def _export(monkeypatch, source, target):
+    from weights_conversion import megatron_to_hf
+
+    monkeypatch.setattr(sys, "argv", [
+        "megatron_to_hf.py", "--input_dir", str(source), "--output_dir",
+        str(target), "--vocab_size", "128"])
+    megatron_to_hf.main()
+
+
+@pytest.mark.parametrize("rotary", ROTARY, ids=lambda r: "-".join(
+    str(x) for x in r.values()))
+def test_export_keeps_rotary_settings(dist_single, tmp_path, monkeypatch,
+                                      rotary):
+    """The exported model, read by another implementation, gives the same
+    logits (fp32, the gate of the other conversions)."""
+    from transformers import AutoModelForCausalLM
+
+    from megatron_amd.utils import get_ltor_masks_and_position_ids
+
+    ours = _checkpoint_of(tmp_path / "in", **rotary)
+    _export(monkeypatch, tmp_path / "in", tmp_path / "out")
+    theirs = AutoModelForCausalLM.from_pretrained(
+        str(tmp_path / "out"), dtype=torch.float32).eval()
+    tokens = torch.randint(0, 128, (2, 32))
+    mask, _, ids = get_ltor_masks_and_position_ids(tokens, 0, False, False,
+                                                   False)
+    with torch.no_grad():
+        want = ours(tokens, ids, mask)[:, :, :128]
+        got = theirs(tokens).logits
+    assert (got - want).abs().max() < 1e-3
+
+
+@pytest.mark.parametrize("rotary", [
+    dict(rotary_percent=0.5),
+    dict(rotary_percent=0.5, rotary_layout="half"),
+])
+def test_export_refuses_what_it_cannot_express(dist_single, tmp_path,
+                                               monkeypatch, rotary):
+    _checkpoint_of(tmp_path / "in", **rotary)
+    with pytest.raises(ValueError, match="rotary_percent"):
+        _export(monkeypatch, tmp_path / "in", tmp_path / "out")
+    assert not (tmp_path / "out").exists()
+
+
+def test_falcon_export_of_halves_moves_no_rows():
+    """Rows are permuted back from the interleaved layout only."""
+    from weights_conversion.megatron_to_hf import megatron_to_hf_falcon
+
+    torch.manual_seed(14)
+    layer = "encoder.layers.0."
+    sd = {layer + name: torch.randn(4) for name in (
+        "input_layernorm.weight", "input_layernorm.bias")}
+    sd.update({layer + name: torch.randn(*shape) for name, shape in (
+        ("self_attention.query_key_value.weight", (96, 64)),
+        ("self_attention.dense.weight", (64, 64)),
+        ("mlp.dense_h_to_4h.weight", (256, 64)),
+        ("mlp.dense_4h_to_h.weight", (64, 256)))})
+    sd.update({"embedding.word_embeddings.weight": torch.randn(128, 64),
+               "encoder.final_layernorm.weight": torch.randn(64),
+               "encoder.final_layernorm.bias": torch.randn(64)})
+    rows = sd[layer + "self_attention.query_key_value.weight"]
+    name = "transformer.h.0.self_attention.query_key_value.weight"
+    half = megatron_to_hf_falcon(sd, 1, 64, 4, 1, 128, rotary_layout="half")
+    assert torch.equal(half[name], rows)
+    plain = megatron_to_hf_falcon(sd, 1, 64, 4, 1, 128)
+    assert not torch.equal(plain[name], rows)

@@ -33,11 +33,14 @@ def load_megatron_checkpoint(input_dir: str):
     return state, model
 
 
-def convert_wqkv(qkv_w, n_heads, n_heads_kv, hidden):
+def convert_wqkv(qkv_w, n_heads, n_heads_kv, hidden,
+                 rotary_layout="interleaved"):
     """Split the fused [q...,k,v]-per-group QKV back to separate HF q/k/v
-    (reference megatron_to_hf.py:47-66)."""
+    (reference megatron_to_hf.py:47-66). Rows in the 'half' layout lie as HF's
+    already."""
     head_dim = hidden // n_heads
-    qkv_w = permute_qkv(qkv_w, hidden, n_heads, n_heads_kv, revert=True)
+    if rotary_layout == "interleaved":
+        qkv_w = permute_qkv(qkv_w, hidden, n_heads, n_heads_kv, revert=True)
     n_qs_per_kv = n_heads // n_heads_kv
     n_groups = qkv_w.size(0) // head_dim // (n_qs_per_kv + 2)
     qkv_w = list(torch.split(qkv_w, head_dim, dim=0))
@@ -63,7 +66,8 @@ def convert_ffn(ffn_w, ffn_hidden):
 
 
 def megatron_to_hf_llama(model_sd: dict, num_layers, hidden, n_heads,
-                         n_heads_kv, ffn_hidden, vocab_size):
+                         n_heads_kv, ffn_hidden, vocab_size,
+                         rotary_layout="interleaved"):
     out = {}
     out["model.embed_tokens.weight"] = model_sd[
         "embedding.word_embeddings.weight"
@@ -81,7 +85,7 @@ def megatron_to_hf_llama(model_sd: dict, num_layers, hidden, n_heads,
         ]
         wq, wk, wv = convert_wqkv(
             model_sd[f"{p}.self_attention.query_key_value.weight"],
-            n_heads, n_heads_kv, hidden,
+            n_heads, n_heads_kv, hidden, rotary_layout,
         )
         out[f"{o}.self_attn.q_proj.weight"] = wq
         out[f"{o}.self_attn.k_proj.weight"] = wk
@@ -101,13 +105,15 @@ def megatron_to_hf_llama(model_sd: dict, num_layers, hidden, n_heads,
 
 
 def megatron_to_hf_falcon(model_sd: dict, num_layers, hidden, n_heads,
-                          n_heads_kv, vocab_size):
+                          n_heads_kv, vocab_size,
+                          rotary_layout="interleaved"):
     """Inverse of hf_to_megatron.falcon_to_megatron (reference
     megatron_to_hf.py:333-434): undo the interleaved->rotate_half rotary row
     permutation on q/k and restore the HF key names."""
-    from weights_conversion.hf_to_megatron import _permute_rotary_rows
 
     def unpermute(w, heads):
+        if rotary_layout == "half":
+            return w
         total, cols = w.shape
         d = total // heads
         wv = w.view(heads, d, cols)
@@ -172,6 +178,32 @@ def megatron_to_hf_falcon(model_sd: dict, num_layers, hidden, n_heads,
     return out
 
 
+def hf_rotary_config(margs, head_dim: int) -> dict:
+    """config.json's part on rotary positions, from a checkpoint's args (those
+    of older or converted checkpoints may lack any of them: the defaults)."""
+    percent = getattr(margs, "rotary_percent", 1.0)
+    if percent != 1.0:
+        raise ValueError(
+            f"rotary_percent {percent}: the exported architectures rotate "
+            "whole heads")
+    theta = getattr(margs, "rope_theta", 10000.0)
+    factor = getattr(margs, "rope_scaling_factor", 1.0)
+    kind = getattr(margs, "rope_scaling_type", "linear")
+    if kind == "ntk":
+        # a larger base and nothing else (models/rope.py)
+        if head_dim > 2:
+            theta = theta * factor ** (head_dim / (head_dim - 2))
+    elif kind not in ("linear", "yarn"):
+        raise ValueError(f"rope_scaling_type {kind} has no form in HF")
+    config = {"rope_theta": theta}
+    if kind != "ntk" and factor != 1.0:
+        config["rope_scaling"] = {"rope_type": kind, "factor": factor}
+        if kind == "yarn":
+            config["rope_scaling"]["original_max_position_embeddings"] = (
+                margs.rope_original_max_positions)
+    return config
+
+
 def write_hf_checkpoint(hf_sd: dict, out_dir: str, config: dict,
                         use_safetensors=True):
     out = Path(out_dir)
@@ -209,9 +241,11 @@ def main():
     n_heads_kv = getattr(margs, "num_attention_heads_kv", n_heads) or n_heads
     ffn_hidden = getattr(margs, "ffn_hidden_size")
 
+    rotary = hf_rotary_config(margs, hidden // n_heads)
+
     hf_sd = megatron_to_hf_llama(
         model_sd, num_layers, hidden, n_heads, n_heads_kv, ffn_hidden,
-        args.vocab_size,
+        args.vocab_size, getattr(margs, "rotary_layout", "interleaved"),
     )
     arch = (
         "MistralForCausalLM" if args.model == "mistral" else "LlamaForCausalLM"
@@ -227,6 +261,7 @@ def main():
         "rms_norm_eps": 1e-5,
         "torch_dtype": "bfloat16",
         "model_type": "mistral" if args.model == "mistral" else "llama",
+        **rotary,
     }
     if args.model == "mistral":
         config["sliding_window"] = 4096
