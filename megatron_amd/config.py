@@ -377,8 +377,25 @@ class TrainingConfig:
         assert self.rotary_layout in ("interleaved", "half")
         assert 0.0 < self.rotary_percent <= 1.0
         if self.rope_scaling_type == "yarn":
-            assert self.rope_original_max_positions is not None, (
-                "yarn needs rope_original_max_positions"
+            assert (self.rope_original_max_positions is not None
+                    and self.rope_original_max_positions >= 1), (
+                "yarn needs rope_original_max_positions, a positive one"
+            )
+        # what the rotary tables refuse (models/rope.py), before a model is
+        # built
+        if self.rope_scaling_type != "linear":
+            assert self.rope_scaling_factor >= 1.0, (
+                f"{self.rope_scaling_type} needs a rope_scaling_factor of 1 "
+                "or more"
+            )
+        if (self.rotary_layout != "interleaved" or self.rotary_percent != 1.0
+                or self.rope_scaling_type != "linear"):
+            assert int(self.kv_channels * self.rotary_percent) >= 2, (
+                f"rotary_percent {self.rotary_percent} leaves no pair of "
+                f"{self.kv_channels} values"
+            )
+            assert self.rope_scaling_factor > 0 and self.rope_theta > 1, (
+                "rope_scaling_factor must be positive, rope_theta exceed 1"
             )
         assert self.kv_cache_bits in (4, 16), "kv_cache_bits is 4 or 16"
         if self.attention_sink_size:
@@ -390,6 +407,15 @@ class TrainingConfig:
         if self.kv_cache_bits == 4:
             assert self.pipeline_model_parallel_size == 1, (
                 "kv_cache_bits 4 needs pipeline_model_parallel_size 1"
+            )
+            from .ops.quant_kv import HEAD_DIMS
+
+            assert self.params_dtype in (torch.bfloat16, torch.half), (
+                "kv_cache_bits 4 needs bf16 or fp16"
+            )
+            assert self.kv_channels in HEAD_DIMS, (
+                f"kv_cache_bits 4 needs kv_channels of {HEAD_DIMS}, not "
+                f"{self.kv_channels}"
             )
 
         if self.lr_warmup_fraction is not None:

@@ -316,3 +316,32 @@ def test_captured_steps_keep_the_window(dist_single, rotary, kv_channels):
         size = want[:, at].norm()
         assert (whole[:, at] - want[:, at]).norm() > 2.0 ** -3 * size
         assert (x - want[:, at]).norm() < 2.0 ** -5 * size, at
+
+
+@pytest.mark.parametrize("bad", [
+    dict(kv_cache_bits=4, bf16=False),               # parameters in fp32
+    dict(kv_cache_bits=4, kv_channels=80),
+    dict(kv_cache_bits=4, kv_channels=None, hidden_size=96),  # heads of 24
+    dict(rotary_percent=0.01),                       # no pair of 64 values
+    dict(rotary_percent=0.01, rotary_layout="half"),
+    dict(rope_scaling_type="ntk", rope_scaling_factor=0.5),
+    dict(rope_scaling_type="yarn", rope_scaling_factor=0.5,
+         rope_original_max_positions=32),
+    dict(rope_scaling_type="yarn", rope_scaling_factor=2.0,
+         rope_original_max_positions=0),
+    dict(rotary_layout="half", rope_scaling_factor=0.0),
+    dict(rotary_layout="half", rope_theta=1.0),
+])
+def test_configuration_refuses_what_a_call_would(bad):
+    """Before a model is built, not in its first forward."""
+    from megatron_amd.config import TrainingConfig
+
+    good = dict(num_layers=2, hidden_size=256, num_attention_heads=4,
+                kv_channels=64, seq_length=64, max_position_embeddings=128,
+                micro_batch_size=2, bf16=True)
+    for more in ({}, dict(kv_cache_bits=4), dict(kv_channels=80),
+                 dict(kv_cache_bits=4, bf16=False, fp16=True),
+                 dict(rotary_percent=0.04), dict(bf16=False)):
+        TrainingConfig(**{**good, **more}).finalize()
+    with pytest.raises(AssertionError):
+        TrainingConfig(**{**good, **bad}).finalize()
