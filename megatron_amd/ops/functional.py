@@ -16,6 +16,7 @@ from __future__ import annotations
 
 import math
 import torch
+from torch.autograd import forward_ad
 
 from . import ext as _ext
 
@@ -416,14 +417,33 @@ def _rotate_pair(query, key, cos, sin, positions, interleaved, inverse):
 _ROTARY_TYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 
+def _has_tangent(*tensors):
+    """Whether one of them is dual in forward-mode differentiation."""
+    if getattr(forward_ad, "_current_level", 0) < 0:  # none can be: cheap
+        return False
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None
+               for t in tensors)
+
+
+def _turn(query, key, cos, sin, positions, interleaved, inverse, tracked):
+    """As _rotate_pair, by an autograd node where something asks for one."""
+    turn = (RotaryFunction.apply if tracked or _has_tangent(query, key)
+            else _rotate_pair)
+    return turn(query, key, cos, sin, positions, interleaved, inverse)
+
+
 class RotaryFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, query, key, cos, sin, positions, interleaved, inverse):
         ctx.save_for_backward(cos, sin, positions)
+        ctx.save_for_forward(cos, sin, positions)
         ctx.mode = (interleaved, inverse)
         ctx.set_materialize_grads(False)
-        return _rotate_pair(query, key, cos, sin, positions, interleaved,
-                            inverse)
+        out = _rotate_pair(query, key, cos, sin, positions, interleaved,
+                           inverse)
+        ctx.like = [None if y is None else (y.shape, y.dtype, y.device)
+                    for y in out]
+        return out
 
     @staticmethod
     def backward(ctx, dq, dk):
@@ -431,11 +451,19 @@ class RotaryFunction(torch.autograd.Function):
         if dq is not None or dk is not None:
             cos, sin, positions = ctx.saved_tensors
             interleaved, inverse = ctx.mode
-            turn = (RotaryFunction.apply if torch.is_grad_enabled()
-                    else _rotate_pair)
-            dq, dk = turn(dq, dk, cos, sin, positions, interleaved,
-                          not inverse)
+            dq, dk = _turn(dq, dk, cos, sin, positions, interleaved,
+                           not inverse, torch.is_grad_enabled())
         return dq, dk, None, None, None, None, None
+
+    @staticmethod
+    def jvp(ctx, tq, tk, *_):
+        # linear: tangents turn as their tensors do. Every output needs one.
+        tangents = [
+            t if t is not None or like is None
+            else torch.zeros(like[0], dtype=like[1], device=like[2])
+            for t, like in zip((tq, tk), ctx.like)]
+        return _turn(*tangents, *ctx.saved_tensors, *ctx.mode,
+                     torch.is_grad_enabled())
 
 
 def rotary_embedding(query, key, cos, sin, positions=None, interleaved=True):
@@ -447,7 +475,7 @@ def rotary_embedding(query, key, cos, sin, positions=None, interleaved=True):
     pass through. positions: int64 [b, s], rows of the tables; None means
     0..s-1 in every sequence. interleaved: pairs are (2j, 2j + 1), else
     (j, j + r). Positions outside the tables are refused on the CPU and give
-    NaN on the GPU. Differentiable in query and key."""
+    NaN on the GPU. Differentiable in query and key, backward and forward."""
     shape = query.shape
     if len(shape) != 4:
         raise ValueError("query must be [s, b, heads, head_dim]")
@@ -483,12 +511,9 @@ def rotary_embedding(query, key, cos, sin, positions=None, interleaved=True):
                 int(positions.min()) < 0 or int(positions.max()) >= rows):
             raise ValueError("a position lies outside the tables")
     cos, sin = cos.contiguous(), sin.contiguous()
-    if not torch.is_grad_enabled() or not (
-            query.requires_grad or (key is not None and key.requires_grad)):
-        return _rotate_pair(query, key, cos, sin, positions, interleaved,
-                            False)
-    return RotaryFunction.apply(query, key, cos, sin, positions, interleaved,
-                                False)
+    tracked = torch.is_grad_enabled() and (
+        query.requires_grad or (key is not None and key.requires_grad))
+    return _turn(query, key, cos, sin, positions, interleaved, False, tracked)
 
 
 # ---------------------------------------------------------------------------

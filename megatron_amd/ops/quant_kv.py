@@ -19,7 +19,7 @@ from typing import Optional, Tuple, Union
 import torch
 
 from . import ext as _ext
-from .functional import rotate_reference
+from .functional import _has_tangent, rotate_reference
 
 GROUP = 32
 HELD_MAX = 57344.0
@@ -134,6 +134,8 @@ class QuantKVCache:
                 t is not None and t.requires_grad for t in tensors):
             raise ValueError("the 4-bit cache has no gradient: call it under "
                              "torch.no_grad()")
+        if _has_tangent(*tensors):
+            raise ValueError("the 4-bit cache has no forward-mode derivative")
 
     # -- operations -----------------------------------------------------------
 

@@ -345,3 +345,63 @@ def test_configuration_refuses_what_a_call_would(bad):
         TrainingConfig(**{**good, **more}).finalize()
     with pytest.raises(AssertionError):
         TrainingConfig(**{**good, **bad}).finalize()
+
+
+@pytest.mark.parametrize("interleaved", [True, False])
+def test_rotary_forward_mode(device, interleaved):
+    """Tangents are turned as their tensors are (the rotation is linear), with
+    and without a gradient beside, and through the backward pass."""
+    import torch.autograd.forward_ad as fwd
+
+    from megatron_amd.models.rope import precompute_rotary_tables
+    from megatron_amd.ops import rotary_embedding
+
+    torch.manual_seed(9)
+    q, k, tq, tk, g, tg = (torch.randn(3, 2, n, 24, device=device)
+                           for n in (4, 1, 4, 1, 4, 4))
+    cos, sin = precompute_rotary_tables(16, 9, device=device)
+
+    def turned(a, b):
+        return rotary_embedding(a, b, cos, sin, interleaved=interleaved)
+
+    want_q, want_k = turned(tq, tk)
+    back, = torch.autograd.grad(
+        turned(q.requires_grad_(), None)[0], q, tg)
+    q = q.detach()
+    with fwd.dual_level():
+        both = turned(fwd.make_dual(q, tq), fwd.make_dual(k, tk))
+        assert torch.equal(fwd.unpack_dual(both[0]).tangent, want_q)
+        assert torch.equal(fwd.unpack_dual(both[1]).tangent, want_k)
+        one = turned(fwd.make_dual(q, tq), k)
+        assert torch.equal(fwd.unpack_dual(one[0]).tangent, want_q)
+        none = fwd.unpack_dual(one[1]).tangent
+        assert none is None or not none.any()
+        alone = turned(fwd.make_dual(q, tq), None)
+        assert torch.equal(fwd.unpack_dual(alone[0]).tangent, want_q)
+        with torch.no_grad():
+            quiet = turned(fwd.make_dual(q, tq), k)
+            assert torch.equal(fwd.unpack_dual(quiet[0]).tangent, want_q)
+        leaf = q.clone().requires_grad_()
+        out, _ = turned(fwd.make_dual(leaf, tq), k)
+        assert torch.equal(fwd.unpack_dual(out).tangent, want_q)
+        dq, = torch.autograd.grad(out, leaf, fwd.make_dual(g, tg))
+        assert torch.equal(fwd.unpack_dual(dq).tangent, back)
+
+
+def test_cache_refuses_forward_mode(device):
+    """As it refuses a gradient: no tangent is dropped in silence."""
+    import torch.autograd.forward_ad as fwd
+
+    from megatron_amd.ops import QuantKVCache
+
+    cache = QuantKVCache(8, 1, 1, 32, device=device)
+    x = torch.randn(1, 1, 1, 32, device=device).bfloat16()
+    with fwd.dual_level(), torch.no_grad():
+        dual = fwd.make_dual(x, x)
+        cache.append(x, x, 0)
+        cache.attention(x, 0)
+        for call in (lambda: cache.append(dual, x, 0),
+                     lambda: cache.append(x, dual, 0),
+                     lambda: cache.attention(dual, 0)):
+            with pytest.raises(ValueError):
+                call()
