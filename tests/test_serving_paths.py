@@ -386,6 +386,8 @@ def test_rotary_forward_mode(device, interleaved):
         assert torch.equal(fwd.unpack_dual(out).tangent, want_q)
         dq, = torch.autograd.grad(out, leaf, fwd.make_dual(g, tg))
         assert torch.equal(fwd.unpack_dual(dq).tangent, back)
+    _, out = torch.func.jvp(lambda a, b: turned(a, b), (q, k), (tq, tk))
+    assert torch.equal(out[0], want_q) and torch.equal(out[1], want_k)
 
 
 def test_cache_refuses_forward_mode(device):
