@@ -82,6 +82,10 @@ class MegatronServer:
             if not 0.0 <= min_p <= 1.0:
                 return JSONResponse({"message": "min_p must be in 0..1"},
                                     status_code=400)
+            if min_p and beam_width is not None:
+                return JSONResponse(
+                    {"message": "min_p has no meaning for a beam search"},
+                    status_code=400)
             if min_p and not (0.0 <= temperature < math.inf and top_k >= 0
                               and 0.0 <= top_p <= 1.0):
                 return JSONResponse(

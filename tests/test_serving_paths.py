@@ -407,3 +407,27 @@ def test_cache_refuses_forward_mode(device):
                      lambda: cache.attention(dual, 0)):
             with pytest.raises(ValueError):
                 call()
+
+
+def test_min_p_beside_beams_is_refused():
+    """A beam search draws nothing: min_p beside it would go unheard."""
+    import asyncio
+    import json
+
+    from megatron_amd.inference import server
+
+    app = server.MegatronServer(None)._build_app()
+    endpoint = next(r.endpoint for r in app.routes if r.path == "/api")
+
+    class Request:
+        async def json(self):
+            return dict(prompts=["a"], min_p=0.1, beam_width=2)
+
+    def never(*args, **kw):
+        raise AssertionError("the other ranks were called upon")
+
+    with pytest.MonkeyPatch.context() as patch:
+        patch.setattr(server, "send_do_beam_search", never)
+        answer = asyncio.run(endpoint(Request()))
+    assert answer.status_code == 400
+    assert "min_p" in json.loads(answer.body)["message"]
