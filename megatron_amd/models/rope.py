@@ -9,6 +9,7 @@ application is a fused HIP kernel (ops/csrc/rope.hip) over interleaved pairs.
 from __future__ import annotations
 
 import math
+import weakref
 from typing import Optional
 
 import torch
@@ -80,6 +81,30 @@ def precompute_rotary_tables(dim: int, end: int, theta: float = 10000.0,
         torch.arange(end, dtype=torch.float64, device=inv.device), inv)
     return (angles.cos() * magnitude).float(), (angles.sin()
                                                 * magnitude).float()
+
+
+class RotaryTables:
+    """cos and sin of precompute_rotary_tables, one pair for all layers that
+    ask for the same: at 131072 positions of 64 pairs a pair is 64 MB. It is
+    gone with the last layer that holds it."""
+
+    _held = weakref.WeakValueDictionary()  # by settings and device
+
+    def __init__(self, settings, device):
+        # a layer that trains may come after one that ran in inference mode
+        with torch.inference_mode(False):
+            self.cos, self.sin = precompute_rotary_tables(
+                device=device, **settings)
+        if self.cos.is_cuda:  # layers on other streams may be next
+            torch.cuda.current_stream(self.cos.device).synchronize()
+
+    @classmethod
+    def of(cls, device, **settings):
+        key = (str(device), *sorted(settings.items()))
+        tables = cls._held.get(key)
+        if tables is None:
+            tables = cls._held[key] = cls(settings, device)
+        return tables
 
 
 def apply_rotary_emb(query: torch.Tensor, key: torch.Tensor,

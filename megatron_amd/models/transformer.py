@@ -28,9 +28,9 @@ from .enums import AttnMaskType, AttnType, LayerType
 from .module import MegatronModule
 from .norms import get_norm
 from .rope import (
+    RotaryTables,
     apply_rotary_emb,
     precompute_freqs,
-    precompute_rotary_tables,
 )
 
 
@@ -290,7 +290,8 @@ class ParallelAttention(MegatronModule):
             or cfg.rope_scaling_type != "linear"
         )
         self._rotary_tables = {}  # by device
-        if cfg.position_embedding_type == "rotary":
+        self.rotary = cfg.position_embedding_type == "rotary"
+        if self.rotary and not self.rotary_general:
             cos, sin = precompute_freqs(
                 self.hidden_size_per_attention_head,
                 cfg.max_position_embeddings,
@@ -326,15 +327,16 @@ class ParallelAttention(MegatronModule):
             cfg = self.cfg
             dim = int(self.hidden_size_per_attention_head
                       * cfg.rotary_percent) // 2 * 2
-            self._rotary_tables[device] = precompute_rotary_tables(
-                dim, cfg.max_position_embeddings, theta=cfg.rope_theta,
+            self._rotary_tables[device] = RotaryTables.of(
+                device, dim=dim, end=cfg.max_position_embeddings,
+                theta=cfg.rope_theta,
                 scaling_type=cfg.rope_scaling_type,
                 scaling_factor=cfg.rope_scaling_factor,
                 original_max_position=cfg.rope_original_max_positions
                 or cfg.max_position_embeddings,
-                device=device,
             )
-        return self._rotary_tables[device]
+        tables = self._rotary_tables[device]
+        return tables.cos, tables.sin
 
     def _quant_cache_attend(self, query, key, value, attention_mask,
                             inference_params):
@@ -356,12 +358,11 @@ class ParallelAttention(MegatronModule):
         graph = getattr(ip, "use_graph", False) and sq == 1
         start = ip.graph_pos if graph else ip.sequence_len_offset
         interleaved = self.cfg.rotary_layout == "interleaved"
-        rotary = self.rope_cos is not None
-        if rotary:
+        if self.rotary:
             cos, sin = self._tables(query.device)
 
         if not graph and start == 0 and not (sinks and sq > window):
-            if rotary:
+            if self.rotary:
                 query, key = ops_f.rotary_embedding(
                     query, key, cos, sin, interleaved=interleaved
                 )
@@ -371,7 +372,7 @@ class ParallelAttention(MegatronModule):
 
         with torch.no_grad():
             query, key, value = (t.detach() for t in (query, key, value))
-            if rotary:
+            if self.rotary:
                 query = cache.append(key, value, start, query=query, cos=cos,
                                      sin=sin, interleaved=interleaved)
             else:

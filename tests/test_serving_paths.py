@@ -431,3 +431,33 @@ def test_min_p_beside_beams_is_refused():
         answer = asyncio.run(endpoint(Request()))
     assert answer.status_code == 400
     assert "min_p" in json.loads(answer.body)["message"]
+
+
+def test_layers_share_rotary_tables(dist_single, device):
+    """One pair of tables for all layers alike, and none besides; they serve a
+    training step also where a generation under inference_mode came first, and
+    go with the models that use them."""
+    import gc
+    import weakref
+
+    tokens = torch.zeros(2, 8, dtype=torch.long, device=device)
+    ids = torch.arange(8, device=device).expand(2, 8)
+    model, _ = make_model(device, rotary_layout="half")
+    other, _ = make_model(device, rotary_layout="half", rope_theta=5000.0)
+    with torch.inference_mode():
+        model(tokens, ids, None), other(tokens, ids, None)
+    first, second = (layer.self_attention
+                     for layer in model.language_model.encoder.layers)
+    here = tokens.device
+    for a, b in zip(first._tables(here), second._tables(here)):
+        assert a.data_ptr() == b.data_ptr() and a.dtype == torch.float32
+    strange = other.language_model.encoder.layers[0].self_attention
+    assert not torch.equal(first._tables(here)[0], strange._tables(here)[0])
+    assert not [n for n, _ in model.named_buffers() if "rope" in n]
+    plain, _ = make_model(device)
+    assert [n for n, _ in plain.named_buffers() if "rope" in n]
+    model(tokens, ids, None, labels=tokens).float().mean().backward()
+    gone = weakref.ref(first._tables(here)[0])
+    del model, first, second, a, b
+    gc.collect()
+    assert gone() is None
