@@ -643,7 +643,7 @@ struct AttentionArgs {
   void* out;
   float* part_o;   // [b * heads, chunks, rows, H], unless chunks == 1
   float* part_ml;  // [b * heads, chunks, rows, 2]
-  int n, s, rep, rows, q_blocks, chunks, groups;
+  int n, rep, rows, q_blocks, chunks, groups;
   int* part_per;  // tiles of a chunk
   float scale_log2e;
   long window, sinks;
@@ -1670,7 +1670,6 @@ torch::Tensor quant_kv_attention(std::vector<torch::Tensor> buffers,
   a.q_ns = query.stride(2);
   a.out = out.data_ptr();
   a.n = n;
-  a.s = (int)s;
   a.rep = n / cache.heads;
   TORCH_CHECK(s * a.rep < (1l << 30), "quant_kv: too many queries at once");
   a.rows = (int)s * a.rep;
@@ -1683,7 +1682,7 @@ torch::Tensor quant_kv_attention(std::vector<torch::Tensor> buffers,
   const int tiles = (a.rows + 15) / 16;
   const int mt = tiles == 1 ? 1 : tiles == 2 || cache.h == 256 ? 2 : 4;
   a.q_blocks = (tiles + mt - 1) / mt;
-  a.q_wide = cache.h >= 32 && (unsigned long)a.q % 16 == 0 &&
+  a.q_wide = (unsigned long)a.q % 16 == 0 &&
              a.q_ss % 8 == 0 && a.q_bs % 8 == 0 && a.q_ns % 8 == 0;
   // Workgroups that the card holds at once share the tokens, or, where there
   // are about as many key heads and query blocks, one more for each of those.
