@@ -609,6 +609,13 @@ class ParallelAttention(MegatronModule):
         if use_flash:
             context = self.flash_attention(query, key, value)
         else:
+            window = self._window() if inference_params is not None else 0
+            if (window and sq == 1 and key.shape[0] > window
+                    and self.attention_type == AttnType.self_attn):
+                # a step sees the window's tokens only
+                key, value = key[-window:], value[-window:]
+                if attention_mask is not None:
+                    attention_mask = attention_mask[..., -window:]
             # expand kv heads for the unfused path
             if self.n_rep > 1:
                 key = key.repeat_interleave(self.n_rep, dim=2)

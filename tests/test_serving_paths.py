@@ -461,3 +461,20 @@ def test_layers_share_rotary_tables(dist_single, device):
     del model, first, second, a, b
     gc.collect()
     assert gone() is None
+
+
+@pytest.mark.parametrize("rotary", [dict(), dict(rotary_layout="half")],
+                         ids=["plain", "half"])
+def test_uncaptured_steps_keep_the_window(dist_single, device, rotary):
+    """As the captured ones (tensor parallel generation does not capture)."""
+    torch.manual_seed(10)
+    tokens = torch.randint(1, 99, (2, 32), device=device)
+    model, _ = make_model(device, sliding_window_size=6, init_method_std=0.1,
+                          **rotary)
+    got, _ = steps_of(model, tokens, 20, 32)
+    ids = torch.arange(32, device=device).expand(2, 32)
+    with torch.no_grad():
+        want = model(tokens, ids, None).float()
+    for i, x in enumerate(got):
+        size = want[:, 19 + i].norm()
+        assert (x - want[:, 19 + i]).norm() < 2.0 ** -5 * size, 19 + i
