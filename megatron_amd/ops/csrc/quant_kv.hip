@@ -337,7 +337,9 @@ __device__ __forceinline__ void store_scales(const CacheView& cache,
 // (21 with the head size known at run time only, the borders of codes looked
 // at one by one and the value's load behind the key's; 41 with a row's lanes
 // anywhere and pieces of 16 bits). 44 MB are read and written, 9 us at a
-// copy's rate: 355 instructions a wave, mostly the choice of codes, bound it.
+// copy's rate, and 355 instructions a wave, mostly the choice of codes, issue
+// for about as long. Both would fit side by side; but a wave loads, computes
+// and stores once and waits half of its cycles.
 template <typename T, int H, bool WIDE>
 __global__ __launch_bounds__(256) void append_kernel(CacheView cache,
                                                      AppendSource k,
@@ -606,8 +608,10 @@ __global__ __launch_bounds__(256) void dequantize_kernel(
 //
 // For a bf16 output held keys, held values and weights are operands in fp16,
 // each rounded by a relative 2^-11 at most, under the output's own 2^-8: three
-// bits more than keys and values have in a cache of the model's type. What
-// 32-bit operands would take is in the fp16 path: three products for one. A
+// bits more than keys and values have in a cache of the model's type. Against
+// 64 bits the output is off by 0.0017 of its norm, the plain form by 0.0016 to
+// 0.0017; the fp16 path's three products bring the latter and take 54 us for 44
+// (32 streams of up to 8192 tokens) and 33 for 26.5 (4 of up to 32768). A
 // weight under 2^-21 of the wave's largest is held to 2^-32 of that one
 // (kLift), so that n tokens are off by n 2^-32 of the largest value at most.
 //
@@ -621,8 +625,7 @@ __global__ __launch_bounds__(256) void dequantize_kernel(
 // the time that the tiles take to come from memory; with three waves a SIMD
 // each hides most of the other. Measured (h = 128, bf16): 32 streams of up to
 // 8192 tokens, 8 key heads, 174 MB: 41 to 48 us, 3.6 to 4.2 TB/s; 4 streams of
-// up to 32768, 105 MB: 27 to 31 us. Loads alone take 29 and 22 of those, and a
-// copy reads and writes 4.9 TB/s.
+// up to 32768, 105 MB: 26 to 31 us. Loads alone take 29 and 22 of those.
 
 using h2 = __attribute__((ext_vector_type(2))) _Float16;
 using h8 = __attribute__((ext_vector_type(8))) _Float16;

@@ -14,7 +14,8 @@
 // Memory bounds it: each value is read and written once, at three operations.
 // 4096 x 4 tokens of 64 heads of 128 values in bf16 take 100 us a direction,
 // 5.4 TB/s, a little over what a copy of 2 GB reaches here (4.9); 107 with the
-// loads parted by branches, 350 with a pair a thread.
+// loads parted by branches, 350 with a pair a thread, which is what widths,
+// strides and addresses that do not fill 16 bytes get.
 
 #include "common.h"
 

@@ -14,11 +14,13 @@
 //
 // A row with a NaN, or with no logit above -inf, gives -1.
 //
-// One compute unit does a row, and its operations bound it: 32000 logits in 32
-// bits with top-k 40 take 11 us (1.5 of them the first pass over the row), 64
-// rows of 65024 in 16 bits with all filters 25, 256 rows of 50257 in 32 bits
-// without filters 31, of which the first pass takes 7.5 at 7 TB/s and the sum
-// of the weights 15. Sums bit by bit took 190, 700 and 219.
+// One compute unit does a row, whatever the number of rows, and its passes bound
+// it: 32000 logits in 32 bits with top-k 40 take 11 us (1.5 of them the first
+// pass over the row), 64 rows of 65024 in 16 bits with all filters 27 on a
+// quarter of the card, 256 rows of 50257 in 32 bits without filters 32, of which
+// the first pass takes 7.5 at 7 TB/s and the sum of the weights 15; more than
+// half of the waves' cycles there go by waiting. Sums bit by bit took 190, 700
+// and 219.
 
 #include "common.h"
 

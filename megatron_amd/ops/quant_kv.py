@@ -207,7 +207,11 @@ class QuantKVCache:
         stands at position start + i, has to be appended already, and sees the
         positions up to its own: with `window_size` w the last w of them, its
         own among them, and the first `sink_size`. Returns
-        [s, b, heads * head_dim]."""
+        [s, b, heads * head_dim].
+
+        On the GPU held keys and values and the softmax's weights are operands
+        in fp16 and sums in 32 bits; in an fp16 cache what the operands'
+        rounding left out is added."""
         self._check_no_grad(query)
         device = self.device
         query = self._check_rows(query, "query", device)
